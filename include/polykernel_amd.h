@@ -177,6 +177,104 @@ PK_API int launch_fused_kv_append_attention(const uint16_t *Q, uint16_t *Kc, uin
 PK_API int launch_quantize_int8_per_channel(const uint16_t *W, int8_t *Wq, float *scale, int K, int N,
                                      void *stream);
 
+/* ---- serving from a paged cache ------------------------------------------
+ * No counterpart in the reference, whose cache is one tensor per batch
+ * (kernels/generated/kv_cache_update.cu:67-69).  Head dims are contiguous, every
+ * other axis has a stride, in elements. */
+
+/* Rotation of positions: pair i (dims i and i + dim / 2 of a head, or 2 i and
+ * 2 i + 1 when interleaved) of a head at position p turns by the angle
+ * 2 pi p turns[i]; both outputs are multiplied by `magnitude`.  The angle is
+ * formed in 64 bits, so far positions lose nothing.  Dims from `dim` on pass.
+ * `inverse` turns back by the same angle with the same magnitude: the transposed
+ * map, which is the rotation's gradient. */
+typedef struct pk_rotary {
+  const double *turns; /* device, [dim / 2]: revolutions per position */
+  int dim;             /* rotated dims of a head: even, 0 < dim <= D */
+  int interleaved, inverse;
+  float magnitude;
+} pk_rotary;
+
+/* How pk_rotary_frequencies stretches the frequencies theta_i = base^(-2 i / dim)
+ * of a model trained on `original` positions to `factor` times as many:
+ *   NONE    as they are
+ *   LINEAR  theta / factor
+ *   BASE    base * factor^(dim / (dim - 2)): the slowest pair as LINEAR, the
+ *           fastest as it is
+ *   BANDS   with w = original theta / (2 pi), the turns within the original
+ *           length: w < low: theta / factor; w > high: theta; between them the
+ *           mean with the weight (w - low) / (high - low) on theta
+ *   RAMP    the same two, mixed linearly in the pair's number between the pairs
+ *           that make `high` and `low` turns within the original length (rounded
+ *           outwards and kept within the head); magnitude 0.1 ln(factor) + 1 */
+enum { PK_ROTARY_NONE = 0, PK_ROTARY_LINEAR = 1, PK_ROTARY_BASE = 2, PK_ROTARY_BANDS = 3, PK_ROTARY_RAMP = 4 };
+/* Host: turns[i] = theta_i / (2 pi), i < dim / 2, and the magnitude (may be
+ * NULL).  low < high (turns) and original are used by BANDS and RAMP only. */
+PK_API int pk_rotary_frequencies(int dim, double base, int scaling, double factor, double low, double high,
+                                 double original, double *turns, double *magnitude);
+
+/* out[b,s,h,:] = rotation of x[b,s,h,:] by positions[b * position_stride + s].
+ * Element (b, s, h, d) lies at b * strides[0] + s * strides[1] + h * strides[2] + d.
+ * `out` may be `x` with the same strides; other overlaps are undefined. */
+PK_API int launch_rotary(const uint16_t *x, const int64_t *x_strides, uint16_t *out, const int64_t *out_strides,
+                         const int32_t *positions, int64_t position_stride, int B, int S, int H, int D,
+                         const pk_rotary *rotary, void *stream);
+
+/* Heads of new tokens: element (t, h, d) at data + t * token + h * head + d. */
+typedef struct pk_tokens {
+  uint16_t *data;
+  int64_t token, head;
+} pk_tokens;
+
+/* Keys and values in pages: element (page, head, row, d) of the keys at
+ * k + page * k_page + head * k_head + row * k_row + d; the values likewise. */
+typedef struct pk_paged_cache {
+  uint16_t *k, *v;
+  int64_t k_page, k_head, k_row, v_page, v_head, v_row;
+  int pages, page_size, heads, dim;
+} pk_paged_cache;
+
+/* The new tokens of a batch of sequences, one sequence's behind the other's, and
+ * their places.  Device tables; what they hold is brought into range by the
+ * kernels: token ranges into [0, tokens), lengths into [0, table_width *
+ * page_size]; a page number outside [0, pages) is a page that is not there.
+ * Tokens behind the last sequence's are left alone (in every output). */
+typedef struct pk_paged_batch {
+  const int32_t *page_table; /* [sequences][table_width]: page of position p at p / page_size */
+  int64_t table_stride;      /* elements between the rows of page_table */
+  int table_width;
+  const int32_t *q_start;    /* [sequences + 1] non-decreasing: tokens [q_start[b], q_start[b + 1])
+                              * are sequence b's; NULL: one token each */
+  const int32_t *kv_len;     /* [sequences]: keys of each sequence, the new tokens' among them */
+  int sequences, tokens;
+  int max_q;                 /* about the most new tokens of a sequence (only speed depends on it); 0: unknown */
+} pk_paged_batch;
+
+/* Append: token i of the n new ones of sequence b has position p = kv_len[b] -
+ * n + i; its keys (rotated, where `rotary` is given) and values are written to
+ * row p % page_size of the sequence's page p / page_size.  Where `q` and `q_out`
+ * are given (rotary too), q_out = q rotated by p; q_out may be q.  Tokens at
+ * negative positions or on a page that is not there leave the cache alone.  Two
+ * tokens of one call must not share a row of the cache.  rotary->inverse is not
+ * taken. */
+PK_API int launch_paged_kv_append(const pk_tokens *k, const pk_tokens *v, const pk_tokens *q, const pk_tokens *q_out,
+                                  int q_heads, const pk_paged_cache *cache, const pk_paged_batch *batch,
+                                  const pk_rotary *rotary, void *stream);
+
+/* Attention of the new tokens over the pages, after their append: token i of
+ * sequence b sees keys j <= kv_len[b] - n + i (causal) or all kv_len[b], and
+ * with window > 0 only those above kv_len[b] - n + i - window; q_heads is a
+ * multiple of the cache's heads, query head h reads head h / (q_heads / heads).
+ * o = sum p v / sum p, p = exp(scale q.k - max), fp32 sums; keys that a token
+ * does not see, or on pages that are not there, take no part, whatever they
+ * hold.  A token that sees no key gets zeros.  Any head dim up to 1024.
+ * `workspace` holds pk_paged_attention_workspace_size bytes (0: may be NULL) for
+ * the call's partial results. */
+PK_API size_t pk_paged_attention_workspace_size(int q_heads, const pk_paged_cache *cache, const pk_paged_batch *batch);
+PK_API int launch_paged_attention(const pk_tokens *q, const pk_tokens *out, int q_heads, const pk_paged_cache *cache,
+                                  const pk_paged_batch *batch, float scale, int causal, int window, void *workspace,
+                                  size_t workspace_bytes, void *stream);
+
 /* Config-2 MLP block: y = add(bias(matmul(gelu(bias(matmul(rmsnorm(x, gamma),
  * W1), b1)), W2), b2), x).  x [M,d], W1 [d,F], W2 [F,d].  `workspace` must
  * hold pk_mlp_block_workspace_size(M, d, F) bytes (the normalised rows and the

@@ -51,6 +51,37 @@ class Plan(C.Structure):
                 ("split_steps", C.c_int)]
 
 
+class Rotary(C.Structure):
+    """struct pk_rotary: the rotation of positions."""
+
+    _fields_ = [("turns", C.c_void_p), ("dim", C.c_int), ("interleaved", C.c_int), ("inverse", C.c_int),
+                ("magnitude", C.c_float)]
+
+
+class Tokens(C.Structure):
+    """struct pk_tokens: heads of new tokens, strides in elements."""
+
+    _fields_ = [("data", C.c_void_p), ("token", C.c_int64), ("head", C.c_int64)]
+
+
+class PagedCache(C.Structure):
+    """struct pk_paged_cache: keys and values in pages, strides in elements."""
+
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_page", C.c_int64), ("k_head", C.c_int64),
+                ("k_row", C.c_int64), ("v_page", C.c_int64), ("v_head", C.c_int64), ("v_row", C.c_int64),
+                ("pages", C.c_int), ("page_size", C.c_int), ("heads", C.c_int), ("dim", C.c_int)]
+
+
+class PagedBatch(C.Structure):
+    """struct pk_paged_batch: the new tokens of a batch of sequences and their places."""
+
+    _fields_ = [("page_table", C.c_void_p), ("table_stride", C.c_int64), ("table_width", C.c_int),
+                ("q_start", C.c_void_p), ("kv_len", C.c_void_p), ("sequences", C.c_int), ("tokens", C.c_int),
+                ("max_q", C.c_int)]
+
+
+ROTARY_SCALINGS = ("none", "linear", "base", "bands", "ramp")
+
 PLAN_TILE, PLAN_STREAM, PLAN_RING, PLAN_ODD, PLAN_RAGGED = range(5)
 PLAN_DECODE, PLAN_FLASH, PLAN_FLASH_HALF, PLAN_FLASH_PAIR = range(5, 9)
 
@@ -92,6 +123,13 @@ SIGNATURES = {
     "pk_fused_residual_rmsnorm_config": (I, [P, P, P, P, I, I, F, C.POINTER(Config), P]),
     "pk_fused_softmax_mask_config": (I, [P, P, P, I, I, C.POINTER(Config), P]),
     "launch_quantize_int8_per_channel": (I, [P, P, P, I, I, P]),
+    "pk_rotary_frequencies": (I, [I, D, I, D, D, D, D, P, C.POINTER(D)]),
+    "launch_rotary": (I, [P, P, P, P, P, I64, I, I, I, I, C.POINTER(Rotary), P]),
+    "launch_paged_kv_append": (I, [C.POINTER(Tokens), C.POINTER(Tokens), C.POINTER(Tokens), C.POINTER(Tokens), I,
+                                   C.POINTER(PagedCache), C.POINTER(PagedBatch), C.POINTER(Rotary), P]),
+    "pk_paged_attention_workspace_size": (SZ, [I, C.POINTER(PagedCache), C.POINTER(PagedBatch)]),
+    "launch_paged_attention": (I, [C.POINTER(Tokens), C.POINTER(Tokens), I, C.POINTER(PagedCache),
+                                   C.POINTER(PagedBatch), F, I, I, P, SZ, P]),
     "pk_mlp_block_workspace_size": (SZ, [I, I, I]),
     "launch_mlp_block": (I, [P, P, P, P, P, P, P, I, I, I, F, P, SZ, P]),
     "pk_decode_mlp_int8_workspace_size": (SZ, [I, I, I]),

@@ -238,6 +238,202 @@ def fused_kv_append_attention(q, k_new, v_new, k_cache, v_cache, s_cache: int,
     return out
 
 
+# ---- serving from a paged cache (no counterpart in the reference) ----------------
+def rotary_frequencies(dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0, low: float = 1.0,
+                       high: float = 4.0, original: int = 0, device="cuda") -> Tuple[torch.Tensor, float]:
+    """(turns, magnitude) for `rotary` and `paged_kv_append`: the revolutions per
+    position of each of dim / 2 pairs, in fp64 on `device`, with the frequencies
+    stretched for long contexts as `scaling` says ("none", "linear", "base",
+    "bands", "ramp"; include/polykernel_amd.h, pk_rotary_frequencies)."""
+    if scaling not in _lib.ROTARY_SCALINGS:
+        raise ValueError(f"scaling: one of {_lib.ROTARY_SCALINGS}, got {scaling!r}")
+    turns = torch.empty(max(dim // 2, 0), dtype=torch.float64)
+    mag = _lib.D()
+    check(_lib.load().pk_rotary_frequencies(dim, base, _lib.ROTARY_SCALINGS.index(scaling), factor, low, high, original,
+                                            turns.data_ptr() or None, mag), "pk_rotary_frequencies")
+    return turns.to(device), mag.value
+
+
+def _heads(t: torch.Tensor, dims: int, name: str) -> None:
+    """A bf16 tensor of heads on the current device: any strides, head dims contiguous."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor")
+    if t.dtype != bf16:
+        raise TypeError(f"{name}: expected {bf16}, got {t.dtype}")
+    if t.dim() != dims:
+        raise ValueError(f"{name}: expected {dims} dimensions, got shape {tuple(t.shape)}")
+    _here(t, name)
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{name}: the head dim must be contiguous (strides {t.stride()})")
+
+
+def _here(t: torch.Tensor, name: str) -> None:
+    if not t.is_cuda:
+        raise ValueError(f"{name}: tensor must live on a GPU (got {t.device})")
+    if t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"{name}: tensor is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _table(t: torch.Tensor, shape, dtype: torch.dtype, name: str) -> int:
+    """A contiguous table of the given shape on the current device."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: expected a torch.Tensor")
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
+    _here(t, name)
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: tensor must be contiguous")
+    return t.data_ptr()
+
+
+def _rotation(turns: torch.Tensor, interleaved: bool, inverse: bool, magnitude: float) -> _lib.Rotary:
+    if isinstance(turns, torch.Tensor) and turns.dim() != 1:
+        raise ValueError(f"turns: expected one dimension, got shape {tuple(turns.shape)}")
+    n = turns.shape[0] if isinstance(turns, torch.Tensor) else 0
+    return _lib.Rotary(_table(turns, (n,), torch.float64, "turns"), 2 * n, int(interleaved), int(inverse), magnitude)
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, turns: torch.Tensor, *, interleaved: bool = False,
+           magnitude: float = 1.0, inverse: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotate the first 2 len(turns) dims of every head by its position: pairs (i, i + len(turns)),
+    or (2 i, 2 i + 1) when `interleaved`, by positions * turns[i] revolutions, times `magnitude`.
+
+    x is [tokens, heads, D] with positions [tokens], or [B, heads, S, D] with positions [S] or
+    [B, S] (int32); any strides with contiguous head dims.  `inverse` rotates back, which is the
+    gradient: dx = rotary(dy, positions, turns, inverse=True).  `out` (contiguous by default) may
+    be `x`."""
+    if not isinstance(x, torch.Tensor) or x.dim() not in (3, 4):
+        raise ValueError("x: expected a tensor [tokens, heads, D] or [B, heads, S, D]")
+    _heads(x, x.dim(), "x")
+    if out is None:
+        out = torch.empty(x.shape, dtype=bf16, device=x.device)
+    else:
+        _heads(out, x.dim(), "out")
+        if out.shape != x.shape:
+            raise ValueError(f"out: expected shape {tuple(x.shape)}, got {tuple(out.shape)}")
+    if x.dim() == 3:
+        S, H, D = x.shape
+        B, per = 1, 0
+        xs, os_ = (0, x.stride(0), x.stride(1)), (0, out.stride(0), out.stride(1))
+        pos = _table(positions, (S,), torch.int32, "positions")
+    else:
+        B, H, S, D = x.shape
+        xs, os_ = (x.stride(0), x.stride(2), x.stride(1)), (out.stride(0), out.stride(2), out.stride(1))
+        whole = isinstance(positions, torch.Tensor) and positions.dim() == 2
+        per = S if whole else 0
+        pos = _table(positions, (B, S) if whole else (S,), torch.int32, "positions")
+    rot = _rotation(turns, interleaved, inverse, magnitude)
+    check(_lib.load().launch_rotary(x.data_ptr(), _strides3(*xs), out.data_ptr(), _strides3(*os_), pos, per, B, S, H, D,
+                                    rot, _stream()), "launch_rotary")
+    return out
+
+
+_strides3 = _lib.I64 * 3
+
+
+def _tokens(t: torch.Tensor, name: str, heads: Optional[int], dim: int, tokens: int) -> _lib.Tokens:
+    _heads(t, 3, name)
+    if t.shape[0] != tokens or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
+        raise ValueError(f"{name}: expected [{tokens}, {'heads' if heads is None else heads}, {dim}], got {tuple(t.shape)}")
+    return _lib.Tokens(t.data_ptr(), t.stride(0), t.stride(1))
+
+
+def _paged(k_cache, v_cache, page_table, q_start, kv_len, tokens: int, max_q: int):
+    _heads(k_cache, 4, "k_cache")
+    _heads(v_cache, 4, "v_cache")
+    if k_cache.shape != v_cache.shape:
+        raise ValueError(f"k_cache and v_cache must have the same shape, got {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
+    pages, heads, page_size, dim = k_cache.shape
+    ks, vs = k_cache.stride(), v_cache.stride()
+    cache = _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], pages,
+                            page_size, heads, dim)
+    if not isinstance(kv_len, torch.Tensor) or kv_len.dim() != 1:
+        raise ValueError("kv_len: expected an int32 tensor [sequences]")
+    B = kv_len.shape[0]
+    if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2 or page_table.shape[0] != B:
+        raise ValueError(f"page_table: expected an int32 tensor [{B}, pages of a sequence]")
+    if page_table.dtype != torch.int32:
+        raise TypeError(f"page_table: expected {torch.int32}, got {page_table.dtype}")
+    _here(page_table, "page_table")
+    if page_table.stride(1) != 1 and page_table.shape[1] > 1:
+        raise ValueError("page_table: the pages of a sequence must be contiguous")
+    if q_start is None and tokens != B:
+        raise ValueError(f"q_start: without it every sequence has one token (got {tokens} tokens, {B} sequences)")
+    batch = _lib.PagedBatch(page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
+                            None if q_start is None else _table(q_start, (B + 1,), torch.int32, "q_start"),
+                            _table(kv_len, (B,), torch.int32, "kv_len"), B, tokens, max_q)
+    return cache, batch
+
+
+def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    page_table: torch.Tensor, q_start: Optional[torch.Tensor], kv_len: torch.Tensor, *,
+                    q: Optional[torch.Tensor] = None, turns: Optional[torch.Tensor] = None, interleaved: bool = False,
+                    magnitude: float = 1.0, q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """Write the new tokens' keys and values into their pages, the keys (and q, which is returned)
+    rotated by their positions on the way where `turns` is given (as in `rotary`).
+
+    k and v [tokens, heads, D] and q [tokens, q heads, D] hold the sequences' new tokens one
+    sequence behind the other: q_start[b] to q_start[b + 1] (int32 [sequences + 1]; None: one token
+    each).  kv_len[b] (int32) counts the sequence's keys with the new ones; the key at position p
+    goes to row p % page_size of page page_table[b, p // page_size] of the caches
+    [pages, heads, page_size, D].  Strides are free as long as head dims are contiguous.  Tokens
+    behind the last sequence's, and tokens on a page number outside the cache, write nothing.
+    `q_out` may be `q`."""
+    T = k.shape[0] if isinstance(k, torch.Tensor) and k.dim() == 3 else 0
+    cache, batch = _paged(k_cache, v_cache, page_table, q_start, kv_len, T, 0)
+    kt, vt = _tokens(k, "k", cache.heads, cache.dim, T), _tokens(v, "v", cache.heads, cache.dim, T)
+    rot = None if turns is None else _rotation(turns, interleaved, False, magnitude)
+    qt = ot = None
+    if q is not None:
+        if rot is None:
+            raise ValueError("q: without turns there is nothing to do for the queries")
+        qt = _tokens(q, "q", None, cache.dim, T)
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=bf16, device=q.device)
+        ot = _tokens(q_out, "q_out", q.shape[1], cache.dim, T)
+    elif q_out is not None:
+        raise ValueError("q_out: there is no q")
+    check(_lib.load().launch_paged_kv_append(kt, vt, qt, ot, 0 if q is None else q.shape[1], cache, batch, rot, _stream()),
+          "launch_paged_kv_append")
+    return q_out
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                    q_start: Optional[torch.Tensor], kv_len: torch.Tensor, *, max_q: Optional[int] = None,
+                    scale: Optional[float] = None, causal: bool = True, window: int = 0,
+                    workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of the new tokens q [tokens, q heads, D] over the pages of their sequences
+    (arguments as `paged_kv_append`, which comes first).  Query head h reads key head
+    h // (q heads / heads).  A token at position p sees the keys up to p (causal) or all kv_len[b],
+    and of them those above p - window (window > 0); one that sees none gets zeros.  `max_q`: the
+    most new tokens of a sequence, as far as known; it is for speed alone.  `out` keeps its rows
+    behind the last sequence's tokens."""
+    T = q.shape[0] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0
+    if max_q is None:
+        B = max(kv_len.shape[0], 1) if isinstance(kv_len, torch.Tensor) and kv_len.dim() else 1
+        max_q = -(-T // B)
+    cache, batch = _paged(k_cache, v_cache, page_table, q_start, kv_len, T, max_q)
+    qt = _tokens(q, "q", None, cache.dim, T)
+    if out is None:
+        out = torch.empty(q.shape, dtype=bf16, device=q.device)
+    ot = _tokens(out, "out", q.shape[1], cache.dim, T)
+    if scale is None:
+        scale = 1.0 / math.sqrt(cache.dim)
+    lib = _lib.load()
+    need = lib.pk_paged_attention_workspace_size(q.shape[1], cache, batch)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    else:
+        _here(workspace, "workspace")
+    check(lib.launch_paged_attention(qt, ot, q.shape[1], cache, batch, scale, int(causal), window,
+                                     None if workspace is None else workspace.data_ptr(),
+                                     0 if workspace is None else workspace.numel() * workspace.element_size(),
+                                     _stream()), "launch_paged_attention")
+    return out
+
+
 def quantize_per_channel(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """quant_golden.quantize_per_channel (quant_golden.py:71-83), bit-exact."""
     K, N = w.shape
