@@ -7,26 +7,11 @@
 #include <algorithm>
 #include <cmath>
 
-#include "paged.hpp"
+#include "paged_decode.hpp"
 
 namespace pk {
 namespace paged {
 namespace {
-
-struct AttendArgs {
-  Heads q, out;
-  Cache cache;
-  Batch batch;
-  int q_heads, causal, window;
-  float c2;  // scale * log2(e)
-};
-
-// The range of keys that new token i of a sequence sees.
-__device__ __forceinline__ void key_range(const AttendArgs &g, const Seq &s, int i, int &lo, int &hi) {
-  const int limit = s.kv - s.n + i + 1;
-  hi = g.causal ? max(0, limit) : s.kv;
-  lo = g.window > 0 && limit > g.window ? limit - g.window : 0;
-}
 
 // Any head dim, stride and alignment: a workgroup per token and query head, its waves
 // on every fourth key, a lane on dims lane, lane + 64, ...; states merged in LDS.
@@ -107,6 +92,71 @@ int run_general(const AttendArgs &g, hipStream_t st) {
   return PK_OK;
 }
 
+// ---- few new tokens per sequence (paged_decode.hpp) ----------------------------
+template <int DP, int MT, bool PAGE16>
+__global__ __launch_bounds__(PD_THREADS, DP == 256 ? 1 : 2) void paged_decode_kernel(DecodeArgs d) {
+  paged_decode_body<DP, MT, PAGE16>(d);
+}
+template <int DP, int MT>
+__global__ __launch_bounds__(PD_THREADS) void paged_decode_merge_kernel(DecodeArgs d) {
+  paged_decode_merge_body<DP, MT>(d);
+}
+
+// The kernel of a call: head dims padded to `dp` (0: the general kernel), 16 mt rows per
+// item, at most `workers` workgroups.
+struct Choice {
+  int dp, mt, workers;
+  size_t workspace() const { return dp && workers > 1 ? 2 * (size_t)workers * pd_part_floats(dp, mt) * sizeof(float) : 0; }
+};
+
+constexpr int PD_LEAST = 4;  // steps of a workgroup
+
+Choice choose(int q_heads, const pk_paged_cache &c, const pk_paged_batch &b) {
+  Choice r{0, 0, 0};
+  if (c.dim > 256 || c.dim % 8 != 0) return r;
+  r.dp = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
+  const int group = q_heads / c.heads;
+  const int64_t rows = (int64_t)std::max(b.max_q, 1) * group;
+  r.mt = rows <= 16 ? 1 : rows <= 32 || r.dp == 256 ? 2 : 4;
+  // no more workgroups than the tables can have work for, nor than run at once
+  const int64_t tiles = (int64_t)b.tokens * group / (16 * r.mt) + b.sequences;
+  const int64_t steps = (int64_t)b.table_width * c.page_size / PD_STEP + 2;
+  const int64_t most = r.dp == 256 ? 256 : 512;
+  const int64_t line = tiles > most * PD_LEAST ? tiles : tiles * steps;  // (products of both stay in 64 bits)
+  r.workers = (int)std::min<int64_t>(most, std::max<int64_t>(1, line * std::min<int64_t>(c.heads, most * PD_LEAST) / PD_LEAST));
+  return r;
+}
+
+bool decode_operands(const AttendArgs &g) {
+  const Cache &c = g.cache;
+  auto rows = [&](int64_t row) { return row >= c.dim && row < (int64_t(1) << 26); };
+  return aligned16(g.q.data) && aligned16(g.out.data) && aligned16(c.k) && aligned16(c.v) &&
+         strides8(g.q.token, g.q.head) && strides8(g.out.token, g.out.head) && strides8(c.k_page, c.k_head, c.k_row) &&
+         strides8(c.v_page, c.v_head, c.v_row) && rows(c.k_row) && rows(c.v_row);
+}
+
+template <int DP, int MT>
+int run_decode_as(const DecodeArgs &d, int workers, hipStream_t st) {
+  if (d.a.cache.page.d % PD_TILE == 0) paged_decode_kernel<DP, MT, true><<<workers, PD_THREADS, 0, st>>>(d);
+  else paged_decode_kernel<DP, MT, false><<<workers, PD_THREADS, 0, st>>>(d);
+  PK_LAUNCH_CHECK("paged_decode_kernel");
+  if (workers > 1) {
+    paged_decode_merge_kernel<DP, MT><<<workers, PD_THREADS, 0, st>>>(d);
+    PK_LAUNCH_CHECK("paged_decode_merge_kernel");
+  }
+  return PK_OK;
+}
+int run_decode(const AttendArgs &g, const Choice &c, void *workspace, hipStream_t st) {
+  const DecodeArgs d{g, static_cast<float *>(workspace), PD_LEAST};
+  if (c.dp == 64) return c.mt == 1   ? run_decode_as<64, 1>(d, c.workers, st)
+                         : c.mt == 2 ? run_decode_as<64, 2>(d, c.workers, st)
+                                     : run_decode_as<64, 4>(d, c.workers, st);
+  if (c.dp == 128) return c.mt == 1   ? run_decode_as<128, 1>(d, c.workers, st)
+                          : c.mt == 2 ? run_decode_as<128, 2>(d, c.workers, st)
+                                      : run_decode_as<128, 4>(d, c.workers, st);
+  return c.mt == 1 ? run_decode_as<256, 1>(d, c.workers, st) : run_decode_as<256, 2>(d, c.workers, st);
+}
+
 }  // namespace
 }  // namespace paged
 }  // namespace pk
@@ -117,15 +167,16 @@ using namespace pk::paged;
 extern "C" {
 
 size_t pk_paged_attention_workspace_size(int q_heads, const pk_paged_cache *cache, const pk_paged_batch *batch) {
-  (void)q_heads, (void)cache, (void)batch;
-  return 0;
+  if (!cache || !batch || q_heads <= 0 || cache->heads <= 0 || q_heads % cache->heads != 0 || cache->dim <= 0 ||
+      cache->page_size <= 0 || batch->tokens <= 0 || batch->sequences <= 0 || batch->table_width < 0)
+    return 0;
+  return choose(q_heads, *cache, *batch).workspace();
 }
 
 int launch_paged_attention(const pk_tokens *q, const pk_tokens *out, int q_heads, const pk_paged_cache *cache,
                            const pk_paged_batch *batch, float scale, int causal, int window, void *workspace,
                            size_t workspace_bytes, void *stream) {
   const char *who = "launch_paged_attention";
-  (void)workspace, (void)workspace_bytes;
   AttendArgs g{};
   if (int rc = check_cache(who, cache, &g.cache)) return rc;
   if (int rc = check_batch(who, batch, cache, &g.batch)) return rc;
@@ -142,7 +193,15 @@ int launch_paged_attention(const pk_tokens *q, const pk_tokens *out, int q_heads
   g.causal = causal != 0;
   g.window = window;
   g.c2 = scale * 1.4426950408889634f;
-  return run_general(g, (hipStream_t)stream);
+  g.group = FastDiv((uint32_t)(q_heads / cache->heads));
+  const Choice c = choose(q_heads, *cache, *batch);
+  // a scale of 0, infinity or no number has no place in the exponents of the fast kernels
+  if (!c.dp || !decode_operands(g) || !(std::fabs(g.c2) > 0.f) || std::isinf(g.c2)) return run_general(g, (hipStream_t)stream);
+  if (workspace_bytes < c.workspace() || (c.workspace() && (!workspace || !aligned16(workspace)))) {
+    set_error("%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who, c.workspace(), workspace_bytes);
+    return PK_ERR_WORKSPACE;
+  }
+  return run_decode(g, c, workspace, (hipStream_t)stream);
 }
 
 }  // extern "C"
