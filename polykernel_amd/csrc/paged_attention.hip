@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "paged_chunk.hpp"
 #include "paged_decode.hpp"
 
 namespace pk {
@@ -92,7 +93,7 @@ int run_general(const AttendArgs &g, hipStream_t st) {
   return PK_OK;
 }
 
-// ---- few new tokens per sequence (paged_decode.hpp) ----------------------------
+// ---- the fast kernels (paged_decode.hpp, paged_chunk.hpp) ------------------------
 template <int DP, int MT, bool PAGE16>
 __global__ __launch_bounds__(PD_THREADS, DP == 256 ? 1 : 2) void paged_decode_kernel(DecodeArgs d) {
   paged_decode_body<DP, MT, PAGE16>(d);
@@ -101,33 +102,66 @@ template <int DP, int MT>
 __global__ __launch_bounds__(PD_THREADS) void paged_decode_merge_kernel(DecodeArgs d) {
   paged_decode_merge_body<DP, MT>(d);
 }
+template <int DP, bool PAGE16>
+__global__ __launch_bounds__(PC_THREADS, DP == 256 ? 1 : 2) void paged_chunk_kernel(ChunkArgs d) {
+  paged_chunk_body<DP, PAGE16>(d);
+}
+template <int DP>
+__global__ __launch_bounds__(PC_THREADS) void paged_chunk_merge_kernel(ChunkArgs d) {
+  paged_chunk_merge_body<DP>(d);
+}
 
-// The kernel of a call: head dims padded to `dp` (0: the general kernel), 16 mt rows per
-// item, at most `workers` workgroups.
+constexpr int PD_LEAST = 4;   // steps of a workgroup
+constexpr int PD_ROWS = 64;   // rows (tokens x heads of a group) of a sequence up to which it is not a chunk
+
+// How a call runs: head dims padded to `dp` (0: by the general kernel); sequences of up to
+// PD_ROWS rows by the decode kernel (mt > 0: 16 mt rows per item, at most `workers`
+// workgroups, items cut between them unless `whole`), sequences of more by the chunk kernel
+// (splits > 0: `items` items at most, each in `splits` runs of keys).  A kernel that runs
+// alone takes all sequences.
 struct Choice {
-  int dp, mt, workers;
-  size_t workspace() const { return dp && workers > 1 ? 2 * (size_t)workers * pd_part_floats(dp, mt) * sizeof(float) : 0; }
+  int dp = 0, mt = 0, workers = 0, whole = 0, splits = 0, items = 0;
+  size_t workspace() const {
+    if (!dp) return 0;
+    const size_t few = mt && workers > 1 && !whole ? 2 * (size_t)workers * pd_part_floats(dp, mt) : 0;
+    const size_t many = splits > 1 ? (size_t)items * splits * pc_part_floats(dp) : 0;
+    return std::max(few, many) * sizeof(float);
+  }
 };
 
-constexpr int PD_LEAST = 4;  // steps of a workgroup
-
 Choice choose(int q_heads, const pk_paged_cache &c, const pk_paged_batch &b) {
-  Choice r{0, 0, 0};
+  Choice r;
   if (c.dim > 256 || c.dim % 8 != 0) return r;
-  r.dp = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
-  const int group = q_heads / c.heads;
-  const int64_t rows = (int64_t)std::max(b.max_q, 1) * group;
-  r.mt = rows <= 16 ? 1 : rows <= 32 || r.dp == 256 ? 2 : 4;
-  // no more workgroups than the tables can have work for, nor than run at once
-  const int64_t tiles = (int64_t)b.tokens * group / (16 * r.mt) + b.sequences;
-  const int64_t steps = (int64_t)b.table_width * c.page_size / PD_STEP + 2;
-  const int64_t most = r.dp == 256 ? 256 : 512;
-  const int64_t line = tiles > most * PD_LEAST ? tiles : tiles * steps;  // (products of both stay in 64 bits)
-  r.workers = (int)std::min<int64_t>(most, std::max<int64_t>(1, line * std::min<int64_t>(c.heads, most * PD_LEAST) / PD_LEAST));
+  const int dp = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
+  const int64_t slots = dp == 256 ? 256 : 512;  // workgroups that run at once
+  const int64_t group = q_heads / c.heads;
+  const int64_t steps = (int64_t)b.table_width * c.page_size / PT_STEP + 2;  // of an item, at most
+  // a hint of fewer tokens than there are on average is none
+  const int64_t most = std::max<int64_t>(b.max_q, ((int64_t)b.tokens + b.sequences - 1) / b.sequences);
+  const bool chunks = most * group > PD_ROWS;
+  // every sequence is a chunk where there is one, or where all have the hint's length
+  const bool few = !chunks || !(b.sequences == 1 || (int64_t)b.max_q * b.sequences == b.tokens);
+  if (chunks) {
+    const int64_t items = ((int64_t)b.tokens * group / PC_ROWS + b.sequences) * c.heads;
+    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({slots / items, steps / 8, 32}));
+    if (items * splits > INT32_MAX) return r;
+    r.items = (int)items;
+    r.splits = (int)splits;
+  }
+  if (few) {
+    const int64_t rows = chunks ? group : most * group;
+    r.mt = rows <= 16 ? 1 : rows <= 32 || dp == 256 ? 2 : 4;
+    // no more workgroups than the tables can have work for
+    const int64_t items = ((int64_t)b.tokens * group / (16 * r.mt) + b.sequences) * c.heads;
+    if (items > INT32_MAX / steps) return r;  // a line of 2^31 steps or more: the general kernel
+    r.whole = steps <= 8;
+    r.workers = (int)std::max<int64_t>(1, std::min(slots, r.whole ? items : items * steps / PD_LEAST));
+  }
+  r.dp = dp;
   return r;
 }
 
-bool decode_operands(const AttendArgs &g) {
+bool tile_operands(const AttendArgs &g) {
   const Cache &c = g.cache;
   auto rows = [&](int64_t row) { return row >= c.dim && row < (int64_t(1) << 26); };
   return aligned16(g.q.data) && aligned16(g.out.data) && aligned16(c.k) && aligned16(c.v) &&
@@ -136,25 +170,37 @@ bool decode_operands(const AttendArgs &g) {
 }
 
 template <int DP, int MT>
-int run_decode_as(const DecodeArgs &d, int workers, hipStream_t st) {
-  if (d.a.cache.page.d % PD_TILE == 0) paged_decode_kernel<DP, MT, true><<<workers, PD_THREADS, 0, st>>>(d);
-  else paged_decode_kernel<DP, MT, false><<<workers, PD_THREADS, 0, st>>>(d);
+int run_decode_as(const DecodeArgs &d, hipStream_t st) {
+  if (d.a.cache.page.d % PT_KEYS == 0) paged_decode_kernel<DP, MT, true><<<d.most, PD_THREADS, 0, st>>>(d);
+  else paged_decode_kernel<DP, MT, false><<<d.most, PD_THREADS, 0, st>>>(d);
   PK_LAUNCH_CHECK("paged_decode_kernel");
-  if (workers > 1) {
-    paged_decode_merge_kernel<DP, MT><<<workers, PD_THREADS, 0, st>>>(d);
+  if (d.most > 1 && !d.whole) {
+    paged_decode_merge_kernel<DP, MT><<<d.most - 1, PD_THREADS, 0, st>>>(d);
     PK_LAUNCH_CHECK("paged_decode_merge_kernel");
   }
   return PK_OK;
 }
-int run_decode(const AttendArgs &g, const Choice &c, void *workspace, hipStream_t st) {
-  const DecodeArgs d{g, static_cast<float *>(workspace), PD_LEAST};
-  if (c.dp == 64) return c.mt == 1   ? run_decode_as<64, 1>(d, c.workers, st)
-                         : c.mt == 2 ? run_decode_as<64, 2>(d, c.workers, st)
-                                     : run_decode_as<64, 4>(d, c.workers, st);
-  if (c.dp == 128) return c.mt == 1   ? run_decode_as<128, 1>(d, c.workers, st)
-                          : c.mt == 2 ? run_decode_as<128, 2>(d, c.workers, st)
-                                      : run_decode_as<128, 4>(d, c.workers, st);
-  return c.mt == 1 ? run_decode_as<256, 1>(d, c.workers, st) : run_decode_as<256, 2>(d, c.workers, st);
+template <int DP>
+int run_as(const AttendArgs &g, const Choice &c, float *workspace, hipStream_t st) {
+  if (c.mt) {
+    const DecodeArgs d{g, workspace, c.whole ? 1 : PD_LEAST, c.workers, c.splits ? PD_ROWS + 1 : INT32_MAX, c.whole};
+    int rc = PK_OK;
+    if (c.mt == 1) rc = run_decode_as<DP, 1>(d, st);
+    else if (c.mt == 2 || DP == 256) rc = run_decode_as<DP, 2>(d, st);
+    else rc = run_decode_as<DP, DP == 256 ? 2 : 4>(d, st);
+    if (rc) return rc;
+  }
+  if (c.splits) {
+    const ChunkArgs d{g, workspace, c.items, c.splits, c.mt ? PD_ROWS : 0};
+    if (g.cache.page.d % PT_KEYS == 0) paged_chunk_kernel<DP, true><<<c.items * c.splits, PC_THREADS, 0, st>>>(d);
+    else paged_chunk_kernel<DP, false><<<c.items * c.splits, PC_THREADS, 0, st>>>(d);
+    PK_LAUNCH_CHECK("paged_chunk_kernel");
+    if (c.splits > 1) {
+      paged_chunk_merge_kernel<DP><<<dim3(c.items, PC_ROWS / PC_MERGE_ROWS), PC_THREADS, 0, st>>>(d);
+      PK_LAUNCH_CHECK("paged_chunk_merge_kernel");
+    }
+  }
+  return PK_OK;
 }
 
 }  // namespace
@@ -196,12 +242,15 @@ int launch_paged_attention(const pk_tokens *q, const pk_tokens *out, int q_heads
   g.group = FastDiv((uint32_t)(q_heads / cache->heads));
   const Choice c = choose(q_heads, *cache, *batch);
   // a scale of 0, infinity or no number has no place in the exponents of the fast kernels
-  if (!c.dp || !decode_operands(g) || !(std::fabs(g.c2) > 0.f) || std::isinf(g.c2)) return run_general(g, (hipStream_t)stream);
+  if (!c.dp || !tile_operands(g) || !(std::fabs(g.c2) > 0.f) || std::isinf(g.c2)) return run_general(g, (hipStream_t)stream);
   if (workspace_bytes < c.workspace() || (c.workspace() && (!workspace || !aligned16(workspace)))) {
     set_error("%s: needs a 16-byte aligned workspace of %zu bytes, got %zu", who, c.workspace(), workspace_bytes);
     return PK_ERR_WORKSPACE;
   }
-  return run_decode(g, c, workspace, (hipStream_t)stream);
+  float *const parts = static_cast<float *>(workspace);
+  return c.dp == 64    ? run_as<64>(g, c, parts, (hipStream_t)stream)
+         : c.dp == 128 ? run_as<128>(g, c, parts, (hipStream_t)stream)
+                       : run_as<256>(g, c, parts, (hipStream_t)stream);
 }
 
 }  // extern "C"

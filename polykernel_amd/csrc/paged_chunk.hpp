@@ -1,0 +1,393 @@
+// paged_chunk.hpp -- attention of many new tokens per sequence over a paged cache.
+//
+// What bounds it: the matrix units and, beside them, the exponentials.  128 rows (token,
+// query head of the group) of one sequence and key head are a workgroup's item, 32 per
+// wave, over steps of 64 keys that the four waves share through LDS.  S^T = K Q^T and
+// O^T = V^T P^T run on v_mfma_f32_32x32x16_bf16 as in the contiguous flash kernel: a lane
+// owns one row and half of the keys, so P never leaves its registers.  P is rounded to
+// bf16 once (half a step, 2^-8 of a weight, its sum kept in fp32): the second product
+// of a low half would be a third of all matrix work.  Two workgroups share a CU, so that
+// one's softmax runs beside the other's products.
+//
+// Items of one key head run next to each other on one XCD and share its L2; a sequence's
+// last rows, which see the most keys, come first.  Few items are also cut into `splits`
+// runs of keys, whose states paged_chunk_merge_kernel adds in order.
+#pragma once
+
+#include "paged_tiles.hpp"
+
+namespace pk {
+namespace paged {
+
+constexpr int PC_WAVES = 4, PC_THREADS = PC_WAVES * 64, PC_ROWS = 32 * PC_WAVES, PC_STEP = PT_STEP;
+
+struct ChunkArgs {
+  AttendArgs a;
+  float *parts;  // splits > 1: [item][split] states
+  int items;     // at most
+  int splits;
+  int above;     // rows of a sequence up to which another kernel takes it
+};
+constexpr size_t pc_part_floats(int DP) { return (size_t)PC_ROWS * (DP + 2); }
+
+// An item: 128 rows of one sequence and key head.
+struct Item {
+  Seq s;
+  int b, hk, tile;
+  int split;
+};
+// Workgroup i's item and split; false behind the last one.  `order`: place of the item
+// on the line of all, for its parts.
+__device__ __forceinline__ bool find_item(const ChunkArgs &d, int splits, int i, bool spread, Item &it, int &order) {
+  const AttendArgs &g = d.a;
+  const int lane = threadIdx.x & 63, B = g.batch.sequences, per = (B + 63) / 64, G = (int)g.group.d;
+  auto tiles_of = [&](const Seq &s) __attribute__((always_inline)) {
+    const int64_t rows = (int64_t)s.n * G;
+    return rows <= d.above ? 0 : (int)((rows + PC_ROWS - 1) / PC_ROWS);
+  };
+  int mine = 0;
+  Seq last{0, 0, 0};
+  for (int k = 0; k < per; ++k) {
+    const int b = lane * per + k;
+    if (b < B) {
+      last = sequence(g.batch, b);
+      mine += tiles_of(last) * g.cache.heads;
+    }
+  }
+  const int incl = wave_scan(mine);
+  const int total = min(__builtin_amdgcn_readlane(incl, 63), d.items);  // (more only where q_start goes down)
+  if (total <= 0 || i / splits >= total) return false;
+  const int v = uniform(spread ? xcd_unit(i, total * splits) : i);
+  const int u = v / splits;  // any place of the item's group: groups are whole runs of splits
+  const uint64_t beyond = __ballot(u < incl);
+  if (beyond == 0) return false;
+  const int l = __ffsll((unsigned long long)beyond) - 1;
+  int at = __builtin_amdgcn_readlane(incl - mine, l), b = l * per, n;
+  for (;; ++b) {
+    if (b >= B) return false;
+    it.s = B > 64 ? sequence(g.batch, b)
+                  : Seq{__builtin_amdgcn_readlane(last.q0, b), __builtin_amdgcn_readlane(last.n, b),
+                        __builtin_amdgcn_readlane(last.kv, b)};
+    n = tiles_of(it.s);
+    if (u < at + n * g.cache.heads) break;
+    at += n * g.cache.heads;
+  }
+  // a sequence's run: heads, of each the splits, of each the tiles from the last one
+  const int in_seq = v - at * splits, per_head = n * splits;
+  if ((unsigned)in_seq >= (unsigned)(per_head * g.cache.heads)) return false;
+  it.b = uniform(b);
+  it.hk = uniform(in_seq / per_head);
+  const int in_head = uniform(in_seq - it.hk * per_head);
+  it.split = uniform(in_head / n);
+  it.tile = n - 1 - (in_head - it.split * n);
+  order = at + it.hk * n + it.tile;
+  return order < d.items;
+}
+
+// A barrier that waits for this wave's LDS accesses and no loads in flight.
+__device__ __forceinline__ void lds_barrier() {
+  lgkm_wait0();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+template <int DP>
+struct ChunkShape {
+  static constexpr int TB = PC_STEP * DP * 2, SL = DP == 64 ? 3 : 2;  // tile bytes, slots of a ring
+  static constexpr int OS = DP * 2 + 16;                             // row stride of a wave's rows on their way out
+  static constexpr int LDS = 2 * SL * TB;
+  static_assert(PC_ROWS * OS <= LDS, "the outputs pass through the rings");
+};
+
+template <int DP, bool PAGE16>
+__device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
+  using S = ChunkShape<DP>;
+  using Tiles = TileLoader<DP, PAGE16, false>;
+  constexpr int CH = DP / 8, TB = S::TB, SL = S::SL, NI = Tiles::NI, DS = DP / 16, DB = DP / 32;
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[S::LDS];
+  __shared__ uint16_t there_s[SL][PC_WAVES];
+  __shared__ int odd_s;
+  const AttendArgs &g = d.a;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wid = uniform(tid >> 6);
+  const int col = lane & 31, h = lane >> 5, gi = lane & 15, grp = lane >> 4;
+  const int D = g.cache.dim, G = (int)g.group.d;
+
+  Item it;
+  int order;
+  if (!find_item(d, d.splits, blockIdx.x, true, it, order)) return;
+  const Seq s = it.s;
+  const int all_rows = s.n * G, row0 = it.tile * PC_ROWS;
+  const int rows = min(PC_ROWS, all_rows - row0);
+  const int wrow = row0 + 32 * wid, wrows = min(32, all_rows - wrow);  // this wave's (may be none)
+
+  // the item's keys, and the keys that all and any of this wave's rows see
+  int lo_first, hi_last, t0, t1;
+  key_range(g, s, (int)g.group.div(row0), lo_first, t0);
+  key_range(g, s, (int)g.group.div(row0 + rows - 1), t1, hi_last);
+  const int klo = lo_first & ~(PT_KEYS - 1);
+  const int steps = max(1, (hi_last - klo + PC_STEP - 1) / PC_STEP);
+  const int s0 = (int)((int64_t)steps * it.split / d.splits), nst = (int)((int64_t)steps * (it.split + 1) / d.splits) - s0;
+  const int kfirst = klo + s0 * PC_STEP;
+  Tiles tiles(g);
+  tiles.begin(g, it.b, it.hk, kfirst + wid * PT_KEYS, nst, hi_last);
+  int lo_any = 0, hi_all = 0, lo_all = 0, hi_any = 0;
+  if (wrows > 0) {
+    key_range(g, s, (int)g.group.div(wrow), lo_any, hi_all);
+    key_range(g, s, (int)g.group.div(wrow + wrows - 1), lo_all, hi_any);
+  }
+
+  // Q^T fragments: row lane % 32, dims 16 ds + 8 h + 0..7
+  int lo, hi;
+  bf16x8 qf[DS];
+  const int my = wrow + min(col, max(wrows, 1) - 1), my_row = min(my, all_rows - 1);
+  const int my_i = (int)g.group.div(my_row);
+  {
+    key_range(g, s, my_i, lo, hi);
+    const uint16_t *qp = g.q.data + (int64_t)(s.q0 + my_i) * g.q.token +
+                         (it.hk * G + my_row - my_i * G) * g.q.head + 8 * h;
+#pragma unroll
+    for (int ds = 0; ds < DS; ++ds) {
+      att::u32x4 v = {0, 0, 0, 0};
+      if (16 * ds + 8 * h < D) v = *reinterpret_cast<const att::u32x4 *>(qp + 16 * ds);
+      if (g.c2 < 0.f) v ^= 0x80008000u;
+      qf[ds] = __builtin_bit_cast(bf16x8, v);
+    }
+  }
+  const float c2 = fabsf(g.c2);
+
+  auto issue = [&](int t) __attribute__((always_inline)) {
+    const int sl = t % SL;
+    tiles.issue(g, t, ring + sl * TB + wid * Tiles::BYTES, ring + (SL + sl) * TB + wid * Tiles::BYTES);
+    const uint32_t is = tiles.there(t);  // by all lanes
+    if (lane == 0) there_s[sl][wid] = (uint16_t)is;
+  };
+
+  f32x16 acc[DB];
+#pragma unroll
+  for (int e = 0; e < DB; ++e)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[e][i] = 0.f;
+  float m_run = -INFINITY, l_run = 0.f;
+  if (tid == 0) odd_s = 0;
+
+#pragma unroll
+  for (int t = 0; t < SL - 1; ++t) issue(t);
+#pragma unroll 1
+  for (int t = 0; t < nst; ++t) {
+    vm_wait<2 * NI * (SL - 2)>();  // this wave's part of step t has landed
+    lds_barrier();                 // and every wave's; nobody reads step t - 1 any more
+    const int sl = t % SL, key = kfirst + t * PC_STEP;
+    uint8_t *const ks = ring + sl * TB, *const vs = ring + (SL + sl) * TB;
+    const uint64_t there = (uint64_t)there_s[sl][0] | (uint64_t)there_s[sl][1] << 16 | (uint64_t)there_s[sl][2] << 32 |
+                           (uint64_t)there_s[sl][3] << 48;
+    const uint32_t there_lo = uniform((int)(uint32_t)there), there_hi = uniform((int)(uint32_t)(there >> 32));
+    issue(t + SL - 1);
+    const bool any = wrows > 0 && key < hi_any && key + PC_STEP > lo_any && (there_lo | there_hi) != 0;
+    const bool whole = (there_lo & there_hi) == 0xFFFFFFFFu;
+    const bool masked = key < lo_all || key + PC_STEP > hi_all || !whole;
+    // the same for every wave: whether some row of the item has a hidden key in this step
+    const bool mixed = key < t1 || key + PC_STEP > t0 || !whole;
+
+    bf16x8 pf[4];
+    uint32_t hid = 0;  // hidden keys of this lane's 32
+    if (any) {
+      f32x16 sc[2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[kb][i] = 0.f;
+        const int row = 32 * kb + col;
+#pragma unroll
+        for (int ds = 0; ds < DS; ++ds) {
+          const att::u32x4 kv = *reinterpret_cast<const att::u32x4 *>(ks + row * DP * 2 + 16 * att::swz_k<CH>(2 * ds + h, row));
+          sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kv), qf[ds], sc[kb], 0, 0, 0);
+        }
+      }
+      if (masked) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int kk = 8 * (i >> 2) + 4 * h + (i & 3), k = key + 32 * kb + kk;
+            if (k < lo || k >= hi || !((kb ? there_hi : there_lo) >> kk & 1)) {
+              sc[kb][i] = -INFINITY;
+              hid |= 1u << (16 * kb + i);
+            }
+          }
+      }
+      float top = sc[0][0];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[kb][i]);
+      top = xor32_max(top);
+      // the maximum in the exponent follows once it is 2^8 behind
+      if (__any((top - m_run) * c2 > 8.f)) {
+        const float m_new = fmaxf(m_run, top);
+        const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - m_new) * c2);
+        m_run = m_new;
+        l_run *= alpha;
+#pragma unroll
+        for (int e = 0; e < DB; ++e) acc[e] *= alpha;
+      }
+      const float mc = m_run == -INFINITY ? 0.f : m_run * c2;
+      float sum = 0.f;
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        att::u32x4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int kb = st >> 1, j = 8 * (st & 1) + 2 * i;
+          const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[kb][j], c2, -mc));
+          const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[kb][j + 1], c2, -mc));
+          sum += p0 + p1;
+          w[i] = pack_bf(p0, p1);
+        }
+        pf[st] = __builtin_bit_cast(bf16x8, w);
+      }
+      l_run += sum;
+    }
+    // A hidden key's value that is no number must not meet its zero weight: the workgroup
+    // multiplies such a step with those values at zero, then with each infinity (a NaN as both
+    // signs) at 2^127 and the keys that a row sees at 2^127: sums overflow to what the row sees.
+    int pass = 3;
+    if (mixed) {
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < TB / (16 * PC_THREADS); ++i) {
+        const att::u32x4 w = *reinterpret_cast<const att::u32x4 *>(vs + 16 * (tid + i * PC_THREADS));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) odd |= word_not_finite(w[e]);
+      }
+      if (__any(odd) && lane == 0) odd_s = 1;
+      lds_barrier();
+      if (uniform(odd_s)) pass = 0;
+    }
+#pragma unroll 1
+    for (;; ++pass) {
+      if (pass < 3) {  // the step's values as they were are kept in the slot of its keys
+        lds_barrier();
+#pragma unroll 1
+        for (int i = 0; i < TB / (16 * PC_THREADS); ++i) {
+          const int x = 16 * (tid + i * PC_THREADS);
+          att::u32x4 w = *reinterpret_cast<const att::u32x4 *>((pass ? ks : vs) + x);
+          if (pass == 0) *reinterpret_cast<att::u32x4 *>(ks + x) = w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = apart_half(w[e], pass) | apart_half(w[e] >> 16, pass) << 16;
+          *reinterpret_cast<att::u32x4 *>(vs + x) = w;
+        }
+        if (tid == 0) odd_s = 0;
+        if (pass > 0) {
+#pragma unroll
+          for (int st = 0; st < 4; ++st) {
+            att::u32x4 w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t two = hid >> (8 * st + 2 * i);
+              w[i] = (two & 1 ? 0u : 0x7F00u) | (two & 2 ? 0u : 0x7F000000u);
+            }
+            pf[st] = __builtin_bit_cast(bf16x8, w);
+          }
+        }
+        lds_barrier();
+      }
+      if (any) {
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+#pragma unroll
+          for (int e = 0; e < DB; ++e) {
+            i16x4 hv[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const int kr = st * 16 + 8 * r + 4 * h + (gi >> 2), dd = e * 32 + 16 * (grp & 1) + 4 * (gi & 3);
+              hv[r] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                  (att::lds_i16x4 *)(vs + kr * DP * 2 + 16 * ((dd >> 3) ^ att::swz_v<DP>(kr)) + 2 * (dd & 7)));
+            }
+            const bf16x8 va = __builtin_bit_cast(bf16x8, __builtin_shufflevector(hv[0], hv[1], 0, 1, 2, 3, 4, 5, 6, 7));
+            acc[e] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pf[st], acc[e], 0, 0, 0);
+          }
+      }
+      if (pass >= 2) break;
+    }
+  }
+  vm_wait<0>();
+  l_run = xor32_sum(l_run);
+
+  if (d.splits > 1) {
+    // this split's state of the rows
+    float *part = d.parts + ((size_t)order * d.splits + it.split) * pc_part_floats(DP);
+    const int r = 32 * wid + col;
+    if (col < wrows) {
+#pragma unroll
+      for (int e = 0; e < DB; ++e)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<f32x4 *>(part + (size_t)r * DP + 32 * e + 8 * j + 4 * h) =
+              f32x4{acc[e][4 * j], acc[e][4 * j + 1], acc[e][4 * j + 2], acc[e][4 * j + 3]};
+      if (h == 0) {
+        part[(size_t)PC_ROWS * DP + 2 * r] = m_run;
+        part[(size_t)PC_ROWS * DP + 2 * r + 1] = l_run;
+      }
+    }
+    return;
+  }
+  // rows in bf16 through LDS, so that a store covers whole rows
+  lds_barrier();
+  uint8_t *const os = ring + wid * 32 * S::OS;
+  const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+#pragma unroll
+  for (int e = 0; e < DB; ++e)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<att::u32x2 *>(os + col * S::OS + 2 * (32 * e + 8 * j + 4 * h)) =
+          att::u32x2{pack_bf(acc[e][4 * j] * inv, acc[e][4 * j + 1] * inv), pack_bf(acc[e][4 * j + 2] * inv, acc[e][4 * j + 3] * inv)};
+  lgkm_wait0();
+#pragma unroll
+  for (int x = 0; x < 32 * CH / 64; ++x) {
+    const int r = (x * 64 + lane) / CH, c = (x * 64 + lane) % CH;
+    if (r < wrows && 8 * c < D) {
+      const int i = (int)g.group.div(wrow + r);
+      *reinterpret_cast<att::u32x4 *>(g.out.data + (int64_t)(s.q0 + i) * g.out.token +
+                                      (it.hk * G + wrow + r - i * G) * g.out.head + 8 * c) =
+          *reinterpret_cast<const att::u32x4 *>(os + r * S::OS + 16 * c);
+    }
+  }
+}
+
+// Adds the splits of an item's rows [16 y, + 16) in order, 4 dims of a row per thread.
+constexpr int PC_MERGE_ROWS = 16;
+template <int DP>
+__device__ __forceinline__ void paged_chunk_merge_body(const ChunkArgs &d) {
+  const AttendArgs &g = d.a;
+  Item it;
+  int order;
+  if (!find_item(d, 1, blockIdx.x, false, it, order)) return;
+  const Seq s = it.s;
+  const int G = (int)g.group.d, D = g.cache.dim, cpr = D / 4;
+  const int row0 = it.tile * PC_ROWS, rows = min(PC_ROWS, s.n * G - row0);
+  const int r0 = blockIdx.y * PC_MERGE_ROWS, n = min(PC_MERGE_ROWS, rows - r0);
+  const float c2 = fabsf(g.c2);
+  const float *parts = d.parts + (size_t)order * d.splits * pc_part_floats(DP);
+  for (int x = threadIdx.x; x < n * cpr; x += PC_THREADS) {
+    const int r = r0 + x / cpr, dd = 4 * (x % cpr);
+    float M = -INFINITY, L = 0.f;
+    for (int k = 0; k < d.splits; ++k) M = fmaxf(M, parts[k * pc_part_floats(DP) + (size_t)PC_ROWS * DP + 2 * r]);
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < d.splits; ++k) {
+      const float *p = parts + k * pc_part_floats(DP);
+      const float m = p[(size_t)PC_ROWS * DP + 2 * r];
+      if (m == -INFINITY && p[(size_t)PC_ROWS * DP + 2 * r + 1] == 0.f) continue;
+      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - M) * c2);
+      L += p[(size_t)PC_ROWS * DP + 2 * r + 1] * f;
+      v += *reinterpret_cast<const f32x4 *>(p + (size_t)r * DP + dd) * f;
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const int i = (int)g.group.div(row0 + r);
+    *reinterpret_cast<att::u32x2 *>(g.out.data + (int64_t)(s.q0 + i) * g.out.token + (it.hk * G + row0 + r - i * G) * g.out.head + dd) =
+        att::u32x2{pack_bf(v[0] * inv, v[1] * inv), pack_bf(v[2] * inv, v[3] * inv)};
+  }
+}
+
+}  // namespace paged
+}  // namespace pk

@@ -24,77 +24,67 @@
 // paged_decode_merge_kernel adds them in the order of the workgroups.
 #pragma once
 
-#include "attention_decode.hpp"
-#include "paged.hpp"
+#include "paged_tiles.hpp"
 
 namespace pk {
 namespace paged {
 
-using att::bf16x8;
-using att::f32x4;
-using att::i16x4;
-
-struct AttendArgs {
-  Heads q, out;
-  Cache cache;
-  Batch batch;
-  int q_heads, causal, window;
-  float c2;  // scale * log2(e)
-  FastDiv group;  // query heads per key head
-};
-
-// The range of keys that new token i of a sequence sees.
-__device__ __forceinline__ void key_range(const AttendArgs &g, const Seq &s, int i, int &lo, int &hi) {
-  const int limit = s.kv - s.n + i + 1;
-  hi = g.causal ? max(0, limit) : s.kv;
-  lo = g.window > 0 && limit > g.window ? limit - g.window : 0;
-}
-
-constexpr int PD_WAVES = 4, PD_THREADS = PD_WAVES * 64, PD_TILE = 16, PD_STEP = PD_WAVES * PD_TILE;
+constexpr int PD_WAVES = 4, PD_THREADS = PD_WAVES * 64, PD_TILE = PT_KEYS, PD_STEP = PT_STEP;
 
 // Bytes of one workgroup's partial state: 16 MT rows of DP sums, and (maximum, sum).
 constexpr size_t pd_part_floats(int DP, int MT) { return (size_t)16 * MT * (DP + 2); }
 
 struct DecodeArgs {
   AttendArgs a;
-  float *parts;      // two partial states per workgroup
-  int least;         // steps per workgroup, where there are enough for all
+  float *parts;  // two partial states per workgroup
+  int least;     // steps per workgroup, where there are enough for all
+  int most;      // workgroups
+  int below;     // rows of a sequence from which on another kernel takes it
+  int whole;     // items are not cut: a step of the line is an item
 };
 
-// A value that every lane of the wave holds, in scalar registers.
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ int64_t uniform(int64_t v) {
-  return (int64_t)((uint64_t)(uint32_t)uniform((int)(uint32_t)v) | (uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32);
-}
-
-// The line of steps: what sequence b adds, and a place on it.
+// The line of steps: what sequence b adds, and a place on it.  The host has made sure
+// that the whole line is below 2^31; a q_start that goes down can make it longer, and
+// then the loops over sequences end at the last one.
 struct Line {
   int tiles, steps, klo;  // row tiles, steps of each item, first key of step 0
-  int64_t units;
+  int unit;               // places of the line that an item takes
+  int units;
 };
 template <int ROWS>
-__device__ __forceinline__ Line line_of(const AttendArgs &g, const Seq &s) {
-  Line l{0, 0, 0, 0};
-  if (s.n <= 0) return l;
+__device__ __forceinline__ Line line_of(const DecodeArgs &d, const Seq &s) {
+  const AttendArgs &g = d.a;
+  Line l{0, 0, 0, 1, 0};
+  if (s.n <= 0 || (int64_t)s.n * (int)g.group.d >= d.below) return l;
   int lo, hi, lo2, hi2;
   key_range(g, s, 0, lo, hi);
   key_range(g, s, s.n - 1, lo2, hi2);
   l.klo = lo & ~(PD_TILE - 1);
   l.tiles = (int)(((int64_t)s.n * (int)g.group.d + ROWS - 1) / ROWS);
   l.steps = max(1, (hi2 - l.klo + PD_STEP - 1) / PD_STEP);
-  l.units = (int64_t)l.tiles * g.cache.heads * l.steps;
+  l.unit = d.whole ? 1 : l.steps;
+  l.units = l.tiles * g.cache.heads * l.unit;
   return l;
 }
 
 struct Place {
-  int64_t total, first, last;  // of the line; this workgroup's part [first, last)
-  int workers;
-  int b;                       // sequence of `first`
-  int64_t in_seq;              // first, from the sequence's own start
-  __device__ __forceinline__ int64_t part(int w) const { return w * total / workers; }
-  // the workgroup whose part unit u is in
-  __device__ __forceinline__ int worker_of(int64_t u) const { return (int)(((u + 1) * workers - 1) / total); }
+  int total, each, more;  // of the line; workgroups get `each` steps, the first `more` one more
+  int workers, first, last;
+  int b, in_seq;          // sequence of `first`, and first from that sequence's own start
+  Seq mine;               // this lane's sequence, where there are at most 64
+  __device__ __forceinline__ int part(int w) const { return w * each + min(w, more); }
+  // the workgroup whose part place u is in
+  __device__ __forceinline__ int worker_of(int u) const {
+    const int wide = more * (each + 1);
+    return u < wide ? u / (each + 1) : more + (u - wide) / each;
+  }
 };
+// Sequence b of the batch: from the lane that read it, or from memory.
+__device__ __forceinline__ Seq sequence_at(const Batch &g, const Place &p, int b) {
+  if (g.sequences > 64) return sequence(g, b);
+  return Seq{__builtin_amdgcn_readlane(p.mine.q0, b), __builtin_amdgcn_readlane(p.mine.n, b),
+             __builtin_amdgcn_readlane(p.mine.kv, b)};
+}
 // Where workgroup w's part begins, found by every wave for itself: lane l adds up the
 // sequences [l, l + 1) * ceil(B / 64), and a scan over the lanes gives each its offset.
 template <int ROWS>
@@ -102,39 +92,42 @@ __device__ __forceinline__ bool find_place(const DecodeArgs &d, int w, Place &p)
   const AttendArgs &g = d.a;
   const int lane = threadIdx.x & 63, B = g.batch.sequences;
   const int per = (B + 63) / 64;
-  int64_t mine = 0;
+  int mine = 0;
+  p.mine = Seq{0, 0, 0};
   for (int i = 0; i < per; ++i) {
     const int b = lane * per + i;
-    if (b < B) mine += line_of<ROWS>(g, sequence(g.batch, b)).units;
+    if (b < B) {
+      p.mine = sequence(g.batch, b);
+      mine += line_of<ROWS>(d, p.mine).units;
+    }
   }
-  int64_t incl = mine;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int64_t up = __shfl_up(incl, o, 64);
-    if (lane >= o) incl += up;
-  }
-  p.total = uniform(__shfl(incl, 63, 64));
-  p.workers = (int)min((int64_t)gridDim.x, max((int64_t)1, p.total / d.least));
-  if (w >= p.workers || p.total == 0) return false;
+  const int incl = wave_scan(mine);
+  p.total = __builtin_amdgcn_readlane(incl, 63);
+  p.workers = min(d.most, max(1, p.total / d.least));
+  if (w >= p.workers || p.total <= 0) return false;
+  p.each = p.total / p.workers;
+  p.more = p.total - p.each * p.workers;
   p.first = p.part(w);
   p.last = p.part(w + 1);
-  const uint64_t holds = __ballot(p.first >= incl - mine && p.first < incl);
-  const int l = __ffsll((unsigned long long)holds) - 1;
-  int64_t at = uniform(__shfl(incl - mine, l, 64));
-  int b = uniform(l * per);
+  const uint64_t beyond = __ballot(p.first < incl);
+  if (beyond == 0) return false;
+  const int l = __ffsll((unsigned long long)beyond) - 1;
+  int at = __builtin_amdgcn_readlane(incl - mine, l), b = l * per;
   for (;; ++b) {
-    const int64_t n = line_of<ROWS>(g, sequence(g.batch, b)).units;
-    if (p.first < at + n) break;
+    if (b >= B) return false;
+    const int n = line_of<ROWS>(d, sequence_at(g.batch, p, b)).units;
+    if (p.first < at + n) {
+      p.b = uniform(b);
+      p.in_seq = uniform(p.first - at);
+      return (unsigned)p.in_seq < (unsigned)n;
+    }
     at += n;
   }
-  p.b = b;
-  p.in_seq = p.first - at;
-  return true;
 }
 
 template <int DP>
 struct DecodeShape {
-  static constexpr int CH = DP / 8, RPI = 1024 / (2 * DP), NI = PD_TILE / RPI, TB = PD_TILE * DP * 2;
+  static constexpr int NI = TileLoader<DP, true, true>::NI, TB = TileLoader<DP, true, true>::BYTES;
   static constexpr int SL = DP == 64 ? 4 : 2;
   static constexpr int WAVE = 2 * SL * TB;  // ring of a wave
   static constexpr int PS = DP + 4;         // row stride of a state in LDS, floats
@@ -142,38 +135,10 @@ struct DecodeShape {
   static_assert(STATE + 64 * 8 <= WAVE, "a wave's state lies in its ring");
 };
 
-// 16 zero bytes that rows which are not there are read from.
-__device__ const uint32_t pd_zeros[4] __attribute__((aligned(16))) = {0, 0, 0, 0};
-
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-// global_load_lds_dwordx4: lane i copies 16 bytes from its own address to lds + 16 i
-// (ordered by vm_wait, as dma_lds16).
-__device__ __forceinline__ void dma_lds16_at(const void *src, const void *lds) {
-  const int m0 = __builtin_amdgcn_readfirstlane((int)(uint32_t)reinterpret_cast<uintptr_t>((lds_void *)lds));
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m0), "v"(src) : "memory", "m0");
-}
-#pragma clang diagnostic pop
-
-// `n` such that a bit pattern is no number or infinite in either half of a word.
-__device__ __forceinline__ bool word_not_finite(uint32_t w) {
-  return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
-}
-
-// A value (low half of w) for the passes over a tile with values that are no numbers: 0
-// keeps the finite ones, 1 and 2 hold 2^127 and -2^127 where it is +inf and -inf, both
-// for a NaN.
-__device__ __forceinline__ uint32_t apart_half(uint32_t w, int pass) {
-  const bool finite = (w & 0x7F80u) != 0x7F80u, nan = !finite && (w & 0x7Fu);
-  if (pass == 0) return finite ? w & 0xFFFFu : 0u;
-  if (pass == 1) return nan || (w & 0xFFFFu) == 0x7F80u ? 0x7F00u : 0u;
-  return nan || (w & 0xFFFFu) == 0xFF80u ? 0xFF00u : 0u;
-}
-
 template <int DP, int MT, bool PAGE16>
 __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
   using S = DecodeShape<DP>;
-  constexpr int CH = S::CH, RPI = S::RPI, NI = S::NI, TB = S::TB, SL = S::SL, PS = S::PS;
+  constexpr int CH = DP / 8, NI = S::NI, TB = S::TB, SL = S::SL, PS = S::PS;
   constexpr int ROWS = 16 * MT, KS = DP / 32, DB = DP / 16;
   // many query fragments are read from LDS at each tile (the waves share them), few stay in registers
   constexpr bool QLDS = MT * KS > 8;
@@ -192,37 +157,31 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
   Place at;
   if (!find_place<ROWS>(d, blockIdx.x, at)) return;
 
-  // source offset of instruction i: row i RPI + lane / CH, swizzled chunk; chunks
-  // behind the head dim lie outside every resource
-  uint32_t kvo[NI], vvo[NI];
-#pragma unroll
-  for (int i = 0; i < NI; ++i) {
-    const int row = i * RPI + lane / CH, sl = lane % CH;
-    const int kc = att::swz_k<CH>(sl, row), vc = sl ^ att::swz_v<DP>(row);
-    kvo[i] = 8 * kc < D ? (uint32_t)(row * (int)g.cache.k_row * 2 + 16 * kc) : 0x80000000u;
-    vvo[i] = 8 * vc < D ? (uint32_t)(row * (int)g.cache.v_row * 2 + 16 * vc) : 0x80000000u;
-  }
-
-  int64_t u = at.first, in_seq = at.in_seq;
-  int b = at.b;
+  TileLoader<DP, PAGE16, true> tiles(g);
+  int u = at.first, in_seq = at.in_seq, b = at.b;
   bool first_segment = true;
-  while (u < at.last) {
-    const Seq s = sequence(g.batch, b);
-    const Line ln = line_of<ROWS>(g, s);
+  while (u < at.last && b < g.batch.sequences) {
+    const Seq s = sequence_at(g.batch, at, b);
+    const Line ln = line_of<ROWS>(d, s);
     if (in_seq >= ln.units) {
       in_seq = 0;
       ++b;
       continue;
     }
-    const int item = (int)(in_seq / ln.steps), st0 = (int)(in_seq - (int64_t)item * ln.steps);
-    const int nst = (int)min((int64_t)(ln.steps - st0), at.last - u);
-    const int hk = item / ln.tiles, tile = item - hk * ln.tiles;
+    const int item = uniform(in_seq / ln.unit), st0 = uniform(in_seq - item * ln.unit);
+    const int took = uniform(min(ln.unit - st0, at.last - u)), nst = d.whole ? ln.steps : took;
+    const int hk = uniform(item / ln.tiles), tile = item - hk * ln.tiles;
     const int row0 = tile * ROWS, rows = min(ROWS, s.n * (int)g.group.d - row0);
 
     // the keys that all rows of the tile see, and those that any does
     int lo_any, hi_all, lo_all, hi_any;
     key_range(g, s, (int)g.group.div(row0), lo_any, hi_all);
     key_range(g, s, (int)g.group.div(row0 + rows - 1), lo_all, hi_any);
+
+    // ---- the wave's tiles: keys [key0 + 64 t, + 16)
+    const int key0 = ln.klo + st0 * PD_STEP + wid * PD_TILE;
+    tiles.begin(g, b, hk, key0, nst, hi_any);  // before the queries' loads: loads return in order
+
     int lo[MT], hi[MT];
     bf16x8 qf[QLDS ? 1 : MT][KS];
     if constexpr (QLDS) {
@@ -253,59 +212,9 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
     }
     const float c2 = fabsf(g.c2);
 
-    // ---- the wave's tiles: keys [key0 + 64 t, + 16)
-    const int key0 = ln.klo + st0 * PD_STEP + wid * PD_TILE;
-    const uint16_t *kbase = g.cache.k + hk * g.cache.k_head, *vbase = g.cache.v + hk * g.cache.v_head;
-    // pages looked up 64 tiles (PAGE16) or 4 tiles (a row a lane) at a time
-    constexpr int BATCH = PAGE16 ? 64 : 4;
-    int pages = -1;
-    auto look_up = [&](int t) __attribute__((always_inline)) {
-      const int key = PAGE16 ? key0 + (t + lane) * PD_STEP : key0 + (t + (lane >> 4)) * PD_STEP + col;
-      pages = key < hi_any ? page_of(g.batch, g.cache, b, key) : -1;
-    };
-    auto keys_of = [&](int t) __attribute__((always_inline)) { return t < nst ? hi_any - (key0 + t * PD_STEP) : 0; };
     auto issue = [&](int t) __attribute__((always_inline)) {
-      if (t % BATCH == 0 && t < nst) look_up(t);
-      const int key = key0 + t * PD_STEP;
-      uint8_t *ks = mine + (t % SL) * TB, *vs = mine + (SL + t % SL) * TB;
-      if constexpr (PAGE16) {
-        const int page = __builtin_amdgcn_readlane(pages, t % BATCH), n = page < 0 ? 0 : min(PD_TILE, keys_of(t));
-        const int row = n > 0 ? key - (int)(g.cache.page.div(key) * g.cache.page.d) : 0;
-        const int64_t pg = n > 0 ? page : 0;
-        const pk_u32x4 kr = rsrc_words(kbase + pg * g.cache.k_page + row * g.cache.k_row,
-                                       n > 0 ? (uint32_t)(((n - 1) * (int)g.cache.k_row + D) * 2) : 0u);
-        const pk_u32x4 vr = rsrc_words(vbase + pg * g.cache.v_page + row * g.cache.v_row,
-                                       n > 0 ? (uint32_t)(((n - 1) * (int)g.cache.v_row + D) * 2) : 0u);
-#pragma unroll
-        for (int i = 0; i < NI; ++i) dma_lds16<true>(kr, ks + i * 1024, kvo[i], 0);
-#pragma unroll
-        for (int i = 0; i < NI; ++i) dma_lds16<true>(vr, vs + i * 1024, vvo[i], 0);
-      } else {
-        const int n = keys_of(t);
-        const uint16_t *kp[NI], *vp[NI];
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-          const int row = i * RPI + lane / CH, sl = lane % CH;
-          const int page = __shfl(pages, (t % BATCH) * 16 + row, 64);
-          const int kc = att::swz_k<CH>(sl, row), vc = sl ^ att::swz_v<DP>(row);
-          const bool there = row < n && page >= 0;
-          const int at_row = there ? key + row - (int)(g.cache.page.div(key + row) * g.cache.page.d) : 0;
-          const uint16_t *zero = reinterpret_cast<const uint16_t *>(pd_zeros);
-          kp[i] = there && 8 * kc < D ? kbase + page * g.cache.k_page + at_row * g.cache.k_row + 8 * kc : zero;
-          vp[i] = there && 8 * vc < D ? vbase + page * g.cache.v_page + at_row * g.cache.v_row + 8 * vc : zero;
-        }
-#pragma unroll
-        for (int i = 0; i < NI; ++i) dma_lds16_at(kp[i], ks + i * 1024);
-#pragma unroll
-        for (int i = 0; i < NI; ++i) dma_lds16_at(vp[i], vs + i * 1024);
-      }
+      tiles.issue(g, t, mine + (t % SL) * TB, mine + (SL + t % SL) * TB);
     };
-    // keys of tile t that are there, a bit each
-    auto there_of = [&](int t, int page_word) __attribute__((always_inline)) -> uint32_t {
-      if constexpr (PAGE16) return __builtin_amdgcn_readlane(page_word, t % BATCH) < 0 ? 0u : 0xFFFFu;
-      else return (uint32_t)(__ballot(page_word >= 0) >> (16 * (t % BATCH))) & 0xFFFFu;
-    };
-
     float m_run[MT], l_run[MT];
     f32x4 acc[MT][DB];
 #pragma unroll
@@ -320,7 +229,7 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
 #pragma unroll
     for (int t = 0; t < SL; ++t) {
       issue(t);
-      there |= (uint64_t)there_of(t, pages) << (16 * t);
+      there |= (uint64_t)tiles.there(t) << (16 * t);
     }
 #pragma unroll 1
     for (int t = 0; t < nst; ++t) {
@@ -444,7 +353,7 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
         }
         lgkm_wait0();  // the slot's reads are done
         issue(t + SL);
-        there = there >> 16 | (uint64_t)there_of(t + SL, pages) << (16 * (SL - 1));
+        there = there >> 16 | (uint64_t)tiles.there(t + SL) << (16 * (SL - 1));
       }
     }
     vm_wait<0>();
@@ -498,53 +407,76 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
       }
       __syncthreads();
     }
-    u += nst;
-    in_seq += nst;
+    u += took;
+    in_seq += took;
     first_segment = false;
   }
 }
 
-// Adds the parts of the item that is cut where workgroup blockIdx.x's part begins, if no
-// earlier workgroup's part begins inside the same item.
+// Adds the parts of an item that is cut between workgroups w0 to w1: the workgroups of
+// this launch numbered w0 + 1 to w1 share its outputs, 4 dims of a row (a chunk) at a
+// time.  A chunk has as many threads as parts (a power of two up to 16), each on every
+// so-many-th part, and their sums meet in LDS.
 template <int DP, int MT>
 __device__ __forceinline__ void paged_decode_merge_body(const DecodeArgs &d) {
   constexpr int ROWS = 16 * MT;
+  __shared__ float sum[PD_THREADS][6];
   const AttendArgs &g = d.a;
-  const int w = blockIdx.x;
-  if (w == 0) return;
+  const int w = blockIdx.x + 1;
   Place at;
   if (!find_place<ROWS>(d, w, at)) return;
-  const Seq s = sequence(g.batch, at.b);
-  const Line ln = line_of<ROWS>(g, s);
-  const int item = (int)(at.in_seq / ln.steps), st = (int)(at.in_seq - (int64_t)item * ln.steps);
-  const int64_t begin = at.first - st;
-  const int w0 = at.worker_of(begin);
-  if (st == 0 || w0 != w - 1) return;
-  const int w1 = at.worker_of(begin + ln.steps - 1);
+  const Seq s = sequence_at(g.batch, at, at.b);
+  const Line ln = line_of<ROWS>(d, s);
+  const int item = uniform(at.in_seq / ln.unit), st = at.in_seq - item * ln.unit;
+  if (st == 0) return;
+  const int begin = at.first - st;
+  const int w0 = uniform(at.worker_of(begin)), w1 = min(uniform(at.worker_of(begin + ln.unit - 1)), at.workers - 1);
   const int hk = item / ln.tiles, tile = item - hk * ln.tiles;
   const int row0 = tile * ROWS, rows = min(ROWS, s.n * (int)g.group.d - row0), D = g.cache.dim;
   const float c2 = fabsf(g.c2);
   const size_t stride = pd_part_floats(DP, MT);
-  // the first workgroup's part is its second one unless it began the item
+  // the first workgroup's part is its second one unless it began with the item
   const float *p0 = d.parts + (size_t)(2 * w0 + (at.part(w0) == begin ? 0 : 1)) * stride;
-  auto part = [&](int k) __attribute__((always_inline)) { return k == w0 ? p0 : d.parts + (size_t)(2 * k) * stride; };
-  for (int x = threadIdx.x; x < rows * (DP / 4); x += PD_THREADS) {
-    const int r = x / (DP / 4), dd = 4 * (x % (DP / 4));
-    if (dd >= D) continue;
+  int groups = 2;
+  while (groups < 16 && groups < w1 - w0 + 1) groups *= 2;
+  const int lanes = PD_THREADS / groups, lane = threadIdx.x & (lanes - 1), grp = threadIdx.x / lanes;
+  const int cpr = D / 4, chunks = rows * cpr;
+  auto weight = [&](float m, float M) __attribute__((always_inline)) {
+    return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - M) * c2);
+  };
+  for (int c0 = (w - w0 - 1) * lanes; c0 < chunks; c0 += (w1 - w0) * lanes) {
+    const int c = min(c0 + lane, chunks - 1), r = c / cpr, dd = 4 * (c - r * cpr);
     float M = -INFINITY, L = 0.f;
-    for (int k = w0; k <= w1; ++k) M = fmaxf(M, part(k)[(size_t)ROWS * DP + 2 * r]);
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int k = w0; k <= w1; ++k) {
-      const float *p = part(k);
-      const float m = p[(size_t)ROWS * DP + 2 * r];
-      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - M) * c2);
-      L += p[(size_t)ROWS * DP + 2 * r + 1] * f;
-      v += *reinterpret_cast<const f32x4 *>(p + (size_t)r * DP + dd) * f;
+    for (int k = w0 + grp; k <= w1; k += groups) {
+      const float *p = k == w0 ? p0 : d.parts + (size_t)(2 * k) * stride;
+      const float m = p[(size_t)ROWS * DP + 2 * r], l = p[(size_t)ROWS * DP + 2 * r + 1];
+      const f32x4 o = *reinterpret_cast<const f32x4 *>(p + (size_t)r * DP + dd);
+      const float M2 = fmaxf(M, m), a = weight(M, M2), f = weight(m, M2);
+      L = L * a + l * f;
+      v = v * a + o * f;
+      M = M2;
     }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    const int i = (int)g.group.div(row0 + r), h = hk * (int)g.group.d + row0 + r - i * (int)g.group.d;
-    *reinterpret_cast<att::u32x2 *>(g.out.data + (int64_t)(s.q0 + i) * g.out.token + h * g.out.head + dd) =
-        att::u32x2{pack_bf(v[0] * inv, v[1] * inv), pack_bf(v[2] * inv, v[3] * inv)};
+    float *x = sum[threadIdx.x];
+    x[0] = M, x[1] = L, x[2] = v[0], x[3] = v[1], x[4] = v[2], x[5] = v[3];
+    __syncthreads();
+    if (grp == 0 && c0 + lane < chunks) {
+      const int n = min(groups, w1 - w0 + 1);
+      for (int k = 1; k < n; ++k) M = fmaxf(M, sum[k * lanes + lane][0]);
+      L = 0.f;
+      v = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int k = 0; k < n; ++k) {
+        const float *y = sum[k * lanes + lane];
+        const float f = weight(y[0], M);
+        L += y[1] * f;
+        v += f32x4{y[2], y[3], y[4], y[5]} * f;
+      }
+      const float inv = L == 0.f ? 0.f : 1.f / L;
+      const int i = (int)g.group.div(row0 + r), h = hk * (int)g.group.d + row0 + r - i * (int)g.group.d;
+      *reinterpret_cast<att::u32x2 *>(g.out.data + (int64_t)(s.q0 + i) * g.out.token + h * g.out.head + dd) =
+          att::u32x2{pack_bf(v[0] * inv, v[1] * inv), pack_bf(v[2] * inv, v[3] * inv)};
+    }
+    __syncthreads();
   }
 }
 

@@ -1,0 +1,158 @@
+// paged_tiles.hpp -- what the two paged attention kernels share: their arguments, lane
+// helpers, and the loads of tiles of 16 keys from pages into LDS.
+#pragma once
+
+#include "attention_decode.hpp"
+#include "paged.hpp"
+
+namespace pk {
+namespace paged {
+
+using att::bf16x8;
+using att::f32x16;
+using att::f32x4;
+using att::i16x4;
+
+struct AttendArgs {
+  Heads q, out;
+  Cache cache;
+  Batch batch;
+  int q_heads, causal, window;
+  float c2;  // scale * log2(e)
+  FastDiv group;  // query heads per key head
+};
+
+// The range of keys that new token i of a sequence sees.
+__device__ __forceinline__ void key_range(const AttendArgs &g, const Seq &s, int i, int &lo, int &hi) {
+  const int limit = s.kv - s.n + i + 1;
+  hi = g.causal ? max(0, limit) : s.kv;
+  lo = g.window > 0 && limit > g.window ? limit - g.window : 0;
+}
+
+// A wave loads tiles of 16 keys, one of every 64 (a step of 4 waves).
+constexpr int PT_KEYS = 16, PT_STEP = 64;
+
+// A value that every lane of the wave holds, in a scalar register.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Inclusive sum over the lanes of a wave: shifts by 1, 2, 4 and 8 inside rows of 16
+// lanes, then the last lane of a row to the next row, and of a half to the other half.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+  return v;
+}
+
+// 16 zero bytes that rows which are not there are read from.
+__device__ const uint32_t pd_zeros[4] __attribute__((aligned(16))) = {0, 0, 0, 0};
+
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+// global_load_lds_dwordx4: lane i copies 16 bytes from its own address to lds + 16 i
+// (ordered by vm_wait, as dma_lds16).
+__device__ __forceinline__ void dma_lds16_at(const void *src, const void *lds) {
+  const int m0 = __builtin_amdgcn_readfirstlane((int)(uint32_t)reinterpret_cast<uintptr_t>((lds_void *)lds));
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m0), "v"(src) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// Direct-to-LDS loads of a wave's tiles: tile t holds keys [key0 + 64 t, + 16) of one key
+// head, 16-byte chunks swizzled for the fragment reads (att::swz_k, att::swz_v).  Keys from
+// `hi` on, keys on pages that are not there and dims behind the head's are zero.
+//
+// A page size that is a multiple of 16 holds a tile in one page (PAGE16): its address is a
+// buffer resource whose length ends the tile, so nothing is computed per lane; 64 tiles'
+// pages are looked up at a time, a lane each.  Other sizes look up a page per row, 4 tiles
+// at a time, and lanes without a row read zeros.  NT: read once, non-temporal.
+template <int DP, bool PAGE16, bool NT>
+struct TileLoader {
+  static constexpr int CH = DP / 8, RPI = 1024 / (2 * DP), NI = PT_KEYS / RPI, BYTES = PT_KEYS * DP * 2;
+  static constexpr int BATCH = PAGE16 ? 64 : 4;
+  uint32_t kvo[NI], vvo[NI];
+  const uint16_t *kbase, *vbase;
+  int b, key0, count, hi, pages;
+
+  // lane's part of instruction i: row i RPI + lane / CH, chunk by its swizzle
+  __device__ __forceinline__ static int row_of(int i) { return i * RPI + (int)(threadIdx.x & 63) / CH; }
+  __device__ __forceinline__ static int k_chunk(int i) { return att::swz_k<CH>((threadIdx.x & 63) % CH, row_of(i)); }
+  __device__ __forceinline__ static int v_chunk(int i) { return (int)((threadIdx.x & 63) % CH) ^ att::swz_v<DP>(row_of(i)); }
+
+  __device__ __forceinline__ explicit TileLoader(const AttendArgs &g) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {  // chunks behind the head dim lie outside every resource
+      kvo[i] = 8 * k_chunk(i) < g.cache.dim ? (uint32_t)(row_of(i) * (int)g.cache.k_row * 2 + 16 * k_chunk(i)) : 0x80000000u;
+      vvo[i] = 8 * v_chunk(i) < g.cache.dim ? (uint32_t)(row_of(i) * (int)g.cache.v_row * 2 + 16 * v_chunk(i)) : 0x80000000u;
+    }
+  }
+  __device__ __forceinline__ void look_up(const AttendArgs &g, int t) {
+    const int lane = threadIdx.x & 63;
+    const int key = key0 + (PAGE16 ? (t + lane) * PT_STEP : (t + (lane >> 4)) * PT_STEP + (lane & 15));
+    pages = key < hi ? page_of(g.batch, g.cache, b, key) : -1;
+  }
+  __device__ __forceinline__ void begin(const AttendArgs &g, int b_, int hk, int key0_, int count_, int hi_) {
+    b = b_, key0 = key0_, count = count_, hi = hi_;
+    kbase = g.cache.k + hk * g.cache.k_head;
+    vbase = g.cache.v + hk * g.cache.v_head;
+    look_up(g, 0);
+  }
+  // Tiles in order from 0; tiles from `count` on load nothing (as many instructions, of no length).
+  __device__ __forceinline__ void issue(const AttendArgs &g, int t, uint8_t *ks, uint8_t *vs) {
+    if (t % BATCH == 0 && t > 0 && t < count) look_up(g, t);
+    const int key = key0 + t * PT_STEP, left = t < count ? hi - key : 0;
+    if constexpr (PAGE16) {
+      const int page = __builtin_amdgcn_readlane(pages, t % BATCH), n = page < 0 ? 0 : min(PT_KEYS, left);
+      const int row = n > 0 ? key - (int)(g.cache.page.div(key) * g.cache.page.d) : 0;
+      const int64_t pg = n > 0 ? page : 0;
+      const pk_u32x4 kr = rsrc_words(kbase + pg * g.cache.k_page + row * g.cache.k_row,
+                                     n > 0 ? (uint32_t)(((n - 1) * (int)g.cache.k_row + g.cache.dim) * 2) : 0u);
+      const pk_u32x4 vr = rsrc_words(vbase + pg * g.cache.v_page + row * g.cache.v_row,
+                                     n > 0 ? (uint32_t)(((n - 1) * (int)g.cache.v_row + g.cache.dim) * 2) : 0u);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) dma_lds16<NT>(kr, ks + i * 1024, kvo[i], 0);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) dma_lds16<NT>(vr, vs + i * 1024, vvo[i], 0);
+    } else {
+      const uint16_t *kp[NI], *vp[NI];
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int row = row_of(i), page = __shfl(pages, (t % BATCH) * 16 + row, 64);
+        const bool is = row < left && page >= 0;
+        const int at = is ? key + row - (int)(g.cache.page.div(key + row) * g.cache.page.d) : 0;
+        const uint16_t *zero = reinterpret_cast<const uint16_t *>(pd_zeros);
+        kp[i] = is && 8 * k_chunk(i) < g.cache.dim ? kbase + page * g.cache.k_page + at * g.cache.k_row + 8 * k_chunk(i) : zero;
+        vp[i] = is && 8 * v_chunk(i) < g.cache.dim ? vbase + page * g.cache.v_page + at * g.cache.v_row + 8 * v_chunk(i) : zero;
+      }
+#pragma unroll
+      for (int i = 0; i < NI; ++i) dma_lds16_at(kp[i], ks + i * 1024);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) dma_lds16_at(vp[i], vs + i * 1024);
+    }
+  }
+  // Which keys of tile t (the last one issued) are on pages that are there, a bit each.
+  __device__ __forceinline__ uint32_t there(int t) const {
+    if constexpr (PAGE16) return __builtin_amdgcn_readlane(pages, t % BATCH) < 0 ? 0u : 0xFFFFu;
+    else return (uint32_t)(__ballot(pages >= 0) >> (16 * (t % BATCH))) & 0xFFFFu;
+  }
+};
+
+// Whether either half of a word is no number or infinite.
+__device__ __forceinline__ bool word_not_finite(uint32_t w) {
+  return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
+}
+
+// A value (low half of w) for the passes over a tile with values that are no numbers: 0
+// keeps the finite ones, 1 and 2 hold 2^127 and -2^127 where it is +inf and -inf, both
+// for a NaN.
+__device__ __forceinline__ uint32_t apart_half(uint32_t w, int pass) {
+  const bool finite = (w & 0x7F80u) != 0x7F80u, nan = !finite && (w & 0x7Fu);
+  if (pass == 0) return finite ? w & 0xFFFFu : 0u;
+  if (pass == 1) return nan || (w & 0xFFFFu) == 0x7F80u ? 0x7F00u : 0u;
+  return nan || (w & 0xFFFFu) == 0xFF80u ? 0xFF00u : 0u;
+}
+
+}  // namespace paged
+}  // namespace pk

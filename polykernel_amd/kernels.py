@@ -254,45 +254,54 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: str = "none", f
     return turns.to(device), mag.value
 
 
-def _heads(t: torch.Tensor, dims: int, name: str) -> None:
-    """A bf16 tensor of heads on the current device: any strides, head dims contiguous."""
+def _device() -> int:
+    if _current_device is None or not torch.cuda.is_initialized():
+        return torch.cuda.current_device() if torch.cuda.is_available() else -2
+    return _current_device()
+
+
+def _elsewhere(t: torch.Tensor, name: str, dev: int) -> Exception:
+    if not t.is_cuda:
+        return ValueError(f"{name}: tensor must live on a GPU (got {t.device})")
+    return ValueError(f"{name}: tensor is on {t.device}, the current device is cuda:{dev}")
+
+
+def _heads(t: torch.Tensor, dims: int, name: str, dev: int) -> Tuple[int, ...]:
+    """The strides of a bf16 tensor of heads on device `dev`: any, with head dims contiguous."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch.Tensor")
     if t.dtype != bf16:
         raise TypeError(f"{name}: expected {bf16}, got {t.dtype}")
-    if t.dim() != dims:
+    strides = t.stride()
+    if len(strides) != dims:
         raise ValueError(f"{name}: expected {dims} dimensions, got shape {tuple(t.shape)}")
-    _here(t, name)
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
-        raise ValueError(f"{name}: the head dim must be contiguous (strides {t.stride()})")
+    if t.get_device() != dev:
+        raise _elsewhere(t, name, dev)
+    if strides[-1] != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{name}: the head dim must be contiguous (strides {strides})")
+    return strides
 
 
-def _here(t: torch.Tensor, name: str) -> None:
-    if not t.is_cuda:
-        raise ValueError(f"{name}: tensor must live on a GPU (got {t.device})")
-    if t.get_device() != torch.cuda.current_device():
-        raise ValueError(f"{name}: tensor is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
-
-
-def _table(t: torch.Tensor, shape, dtype: torch.dtype, name: str) -> int:
-    """A contiguous table of the given shape on the current device."""
+def _table(t: torch.Tensor, shape, dtype: torch.dtype, name: str, dev: int) -> int:
+    """A contiguous table of the given shape on device `dev`."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch.Tensor")
     if t.dtype != dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
-    _here(t, name)
+    if t.shape != shape:
+        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.get_device() != dev:
+        raise _elsewhere(t, name, dev)
     if not t.is_contiguous():
         raise ValueError(f"{name}: tensor must be contiguous")
     return t.data_ptr()
 
 
-def _rotation(turns: torch.Tensor, interleaved: bool, inverse: bool, magnitude: float) -> _lib.Rotary:
+def _rotation(turns: torch.Tensor, interleaved: bool, inverse: bool, magnitude: float, dev: int) -> _lib.Rotary:
     if isinstance(turns, torch.Tensor) and turns.dim() != 1:
         raise ValueError(f"turns: expected one dimension, got shape {tuple(turns.shape)}")
     n = turns.shape[0] if isinstance(turns, torch.Tensor) else 0
-    return _lib.Rotary(_table(turns, (n,), torch.float64, "turns"), 2 * n, int(interleaved), int(inverse), magnitude)
+    return _lib.Rotary(_table(turns, (n,), torch.float64, "turns", dev), 2 * n, interleaved, inverse, magnitude)
 
 
 def rotary(x: torch.Tensor, positions: torch.Tensor, turns: torch.Tensor, *, interleaved: bool = False,
@@ -306,25 +315,27 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, turns: torch.Tensor, *, int
     be `x`."""
     if not isinstance(x, torch.Tensor) or x.dim() not in (3, 4):
         raise ValueError("x: expected a tensor [tokens, heads, D] or [B, heads, S, D]")
-    _heads(x, x.dim(), "x")
+    dev, dims = _device(), x.dim()
+    xs = _heads(x, dims, "x", dev)
     if out is None:
         out = torch.empty(x.shape, dtype=bf16, device=x.device)
+        os_ = out.stride()
     else:
-        _heads(out, x.dim(), "out")
+        os_ = _heads(out, dims, "out", dev)
         if out.shape != x.shape:
             raise ValueError(f"out: expected shape {tuple(x.shape)}, got {tuple(out.shape)}")
-    if x.dim() == 3:
+    if dims == 3:
         S, H, D = x.shape
         B, per = 1, 0
-        xs, os_ = (0, x.stride(0), x.stride(1)), (0, out.stride(0), out.stride(1))
-        pos = _table(positions, (S,), torch.int32, "positions")
+        xs, os_ = (0, xs[0], xs[1]), (0, os_[0], os_[1])
+        pos = _table(positions, (S,), torch.int32, "positions", dev)
     else:
         B, H, S, D = x.shape
-        xs, os_ = (x.stride(0), x.stride(2), x.stride(1)), (out.stride(0), out.stride(2), out.stride(1))
+        xs, os_ = (xs[0], xs[2], xs[1]), (os_[0], os_[2], os_[1])
         whole = isinstance(positions, torch.Tensor) and positions.dim() == 2
         per = S if whole else 0
-        pos = _table(positions, (B, S) if whole else (S,), torch.int32, "positions")
-    rot = _rotation(turns, interleaved, inverse, magnitude)
+        pos = _table(positions, (B, S) if whole else (S,), torch.int32, "positions", dev)
+    rot = _rotation(turns, interleaved, inverse, magnitude, dev)
     check(_lib.load().launch_rotary(x.data_ptr(), _strides3(*xs), out.data_ptr(), _strides3(*os_), pos, per, B, S, H, D,
                                     rot, _stream()), "launch_rotary")
     return out
@@ -333,22 +344,21 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, turns: torch.Tensor, *, int
 _strides3 = _lib.I64 * 3
 
 
-def _tokens(t: torch.Tensor, name: str, heads: Optional[int], dim: int, tokens: int) -> _lib.Tokens:
-    _heads(t, 3, name)
-    if t.shape[0] != tokens or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{name}: expected [{tokens}, {'heads' if heads is None else heads}, {dim}], got {tuple(t.shape)}")
-    return _lib.Tokens(t.data_ptr(), t.stride(0), t.stride(1))
+def _tokens(t: torch.Tensor, name: str, heads: Optional[int], dim: int, tokens: int, dev: int) -> _lib.Tokens:
+    strides = _heads(t, 3, name, dev)
+    shape = t.shape
+    if shape[0] != tokens or shape[2] != dim or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{name}: expected [{tokens}, {'heads' if heads is None else heads}, {dim}], got {tuple(shape)}")
+    return _lib.Tokens(t.data_ptr(), strides[0], strides[1])
 
 
-def _paged(k_cache, v_cache, page_table, q_start, kv_len, tokens: int, max_q: int):
-    _heads(k_cache, 4, "k_cache")
-    _heads(v_cache, 4, "v_cache")
-    if k_cache.shape != v_cache.shape:
-        raise ValueError(f"k_cache and v_cache must have the same shape, got {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
-    pages, heads, page_size, dim = k_cache.shape
-    ks, vs = k_cache.stride(), v_cache.stride()
-    cache = _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], pages,
-                            page_size, heads, dim)
+def _paged(k_cache, v_cache, page_table, q_start, kv_len, tokens: int, max_q: int, dev: int):
+    ks, vs = _heads(k_cache, 4, "k_cache", dev), _heads(v_cache, 4, "v_cache", dev)
+    shape = k_cache.shape
+    if shape != v_cache.shape:
+        raise ValueError(f"k_cache and v_cache must have the same shape, got {tuple(shape)}, {tuple(v_cache.shape)}")
+    cache = _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], shape[0],
+                            shape[2], shape[1], shape[3])
     if not isinstance(kv_len, torch.Tensor) or kv_len.dim() != 1:
         raise ValueError("kv_len: expected an int32 tensor [sequences]")
     B = kv_len.shape[0]
@@ -356,15 +366,18 @@ def _paged(k_cache, v_cache, page_table, q_start, kv_len, tokens: int, max_q: in
         raise ValueError(f"page_table: expected an int32 tensor [{B}, pages of a sequence]")
     if page_table.dtype != torch.int32:
         raise TypeError(f"page_table: expected {torch.int32}, got {page_table.dtype}")
-    _here(page_table, "page_table")
-    if page_table.stride(1) != 1 and page_table.shape[1] > 1:
+    if page_table.get_device() != dev:
+        raise _elsewhere(page_table, "page_table", dev)
+    ts, width = page_table.stride(), page_table.shape[1]
+    if ts[1] != 1 and width > 1:
         raise ValueError("page_table: the pages of a sequence must be contiguous")
-    if q_start is None and tokens != B:
-        raise ValueError(f"q_start: without it every sequence has one token (got {tokens} tokens, {B} sequences)")
-    batch = _lib.PagedBatch(page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
-                            None if q_start is None else _table(q_start, (B + 1,), torch.int32, "q_start"),
-                            _table(kv_len, (B,), torch.int32, "kv_len"), B, tokens, max_q)
-    return cache, batch
+    if q_start is None:
+        if tokens != B:
+            raise ValueError(f"q_start: without it every sequence has one token (got {tokens} tokens, {B} sequences)")
+    else:
+        q_start = _table(q_start, (B + 1,), torch.int32, "q_start", dev)
+    return cache, _lib.PagedBatch(page_table.data_ptr(), ts[0], width, q_start,
+                                  _table(kv_len, (B,), torch.int32, "kv_len", dev), B, tokens, max_q)
 
 
 def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -381,22 +394,24 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     [pages, heads, page_size, D].  Strides are free as long as head dims are contiguous.  Tokens
     behind the last sequence's, and tokens on a page number outside the cache, write nothing.
     `q_out` may be `q`."""
-    T = k.shape[0] if isinstance(k, torch.Tensor) and k.dim() == 3 else 0
-    cache, batch = _paged(k_cache, v_cache, page_table, q_start, kv_len, T, 0)
-    kt, vt = _tokens(k, "k", cache.heads, cache.dim, T), _tokens(v, "v", cache.heads, cache.dim, T)
-    rot = None if turns is None else _rotation(turns, interleaved, False, magnitude)
+    T, dev = k.shape[0] if isinstance(k, torch.Tensor) and k.dim() == 3 else 0, _device()
+    cache, batch = _paged(k_cache, v_cache, page_table, q_start, kv_len, T, 0, dev)
+    heads, D = cache.heads, cache.dim
+    kt, vt = _tokens(k, "k", heads, D, T, dev), _tokens(v, "v", heads, D, T, dev)
+    rot = None if turns is None else _rotation(turns, interleaved, False, magnitude, dev)
     qt = ot = None
+    Hq = 0
     if q is not None:
         if rot is None:
             raise ValueError("q: without turns there is nothing to do for the queries")
-        qt = _tokens(q, "q", None, cache.dim, T)
+        qt = _tokens(q, "q", None, D, T, dev)
+        Hq = q.shape[1]
         if q_out is None:
             q_out = torch.empty(q.shape, dtype=bf16, device=q.device)
-        ot = _tokens(q_out, "q_out", q.shape[1], cache.dim, T)
+        ot = _tokens(q_out, "q_out", Hq, D, T, dev)
     elif q_out is not None:
         raise ValueError("q_out: there is no q")
-    check(_lib.load().launch_paged_kv_append(kt, vt, qt, ot, 0 if q is None else q.shape[1], cache, batch, rot, _stream()),
-          "launch_paged_kv_append")
+    check(_lib.load().launch_paged_kv_append(kt, vt, qt, ot, Hq, cache, batch, rot, _stream()), "launch_paged_kv_append")
     return q_out
 
 
@@ -410,27 +425,32 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     and of them those above p - window (window > 0); one that sees none gets zeros.  `max_q`: the
     most new tokens of a sequence, as far as known; it is for speed alone.  `out` keeps its rows
     behind the last sequence's tokens."""
-    T = q.shape[0] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0
+    T, dev = q.shape[0] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0, _device()
     if max_q is None:
         B = max(kv_len.shape[0], 1) if isinstance(kv_len, torch.Tensor) and kv_len.dim() else 1
         max_q = -(-T // B)
-    cache, batch = _paged(k_cache, v_cache, page_table, q_start, kv_len, T, max_q)
-    qt = _tokens(q, "q", None, cache.dim, T)
+    cache, batch = _paged(k_cache, v_cache, page_table, q_start, kv_len, T, max_q, dev)
+    D = cache.dim
+    qt = _tokens(q, "q", None, D, T, dev)
+    Hq = q.shape[1]
     if out is None:
         out = torch.empty(q.shape, dtype=bf16, device=q.device)
-    ot = _tokens(out, "out", q.shape[1], cache.dim, T)
+    ot = _tokens(out, "out", Hq, D, T, dev)
     if scale is None:
-        scale = 1.0 / math.sqrt(cache.dim)
+        scale = 1.0 / math.sqrt(D)
     lib = _lib.load()
-    need = lib.pk_paged_attention_workspace_size(q.shape[1], cache, batch)
-    if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    ws, room = None, 0
+    if workspace is not None:
+        if workspace.get_device() != dev:
+            raise _elsewhere(workspace, "workspace", dev)
+        ws, room = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     else:
-        _here(workspace, "workspace")
-    check(lib.launch_paged_attention(qt, ot, q.shape[1], cache, batch, scale, int(causal), window,
-                                     None if workspace is None else workspace.data_ptr(),
-                                     0 if workspace is None else workspace.numel() * workspace.element_size(),
-                                     _stream()), "launch_paged_attention")
+        need = lib.pk_paged_attention_workspace_size(Hq, cache, batch)
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+            ws, room = workspace.data_ptr(), need
+    check(lib.launch_paged_attention(qt, ot, Hq, cache, batch, scale, causal, window, ws, room, _stream()),
+          "launch_paged_attention")
     return out
 
 

@@ -22,6 +22,12 @@ def pk():
     return kernels
 
 
+def ok(got, want, bound):
+    """Every value within its bound (a call of its own, so that a failure prints a number)."""
+    bad = ref.far(got, want, bound)
+    assert bad == 0, f"{bad} of {got.numel()} values outside their bounds"
+
+
 def gen(seed):
     return torch.Generator(device="cuda").manual_seed(seed)
 
@@ -76,7 +82,7 @@ def test_rotary_heads_first(pk, B, H, S, D, rot, per_sequence):
     for b in range(B):
         rows = x[b].transpose(0, 1).double()
         want = ref.rotate(rows, pos[b] if per_sequence else pos, turns)
-        assert ref.far(got[b].transpose(0, 1), want, ref.rotate_bound(rows, want, turns)) == 0
+        ok(got[b].transpose(0, 1), want, ref.rotate_bound(rows, want, turns))
 
 
 @pytest.mark.parametrize("offset", [0, 8, 1, 3])  # elements from a 16-byte boundary
@@ -93,7 +99,7 @@ def test_rotary_strides_and_alignment(pk, offset, pad):
     pos = torch.arange(50, 50 + S, device="cuda", dtype=torch.int32)
     pk.rotary(x, pos, turns, out=out)
     want = ref.rotate(x.double(), pos, turns)
-    assert ref.far(out, want, ref.rotate_bound(x.double(), want, turns)) == 0
+    ok(out, want, ref.rotate_bound(x.double(), want, turns))
     out.fill_(7.0)
     assert bool((room == 7.0).all())
 
@@ -127,7 +133,7 @@ def test_rotary_gradient(pk):
         x, dy = normal(g, D, 3, D).double().requires_grad_(), normal(g, D, 3, D)
         ref.rotate(x, pos, turns, interleaved, 1.25).backward(dy.double())
         dx = pk.rotary(dy, pos, turns, interleaved=interleaved, magnitude=1.25, inverse=True)
-        assert ref.far(dx, x.grad, ref.rotate_bound(dy.double(), x.grad, turns, interleaved, 1.25)) == 0
+        ok(dx, x.grad, ref.rotate_bound(dy.double(), x.grad, turns, interleaved, 1.25))
 
 
 # ---- paged caches -------------------------------------------------------------
@@ -195,7 +201,7 @@ def test_append(pk, qs, kvs, Hq, Hkv, D, rot, P, interleaved, rows_first, pad, r
     bound = torch.zeros_like(want_k)
     if rotated:
         want = ref.rotate(q[:T].double(), pos, turns, **kw)
-        assert ref.far(qo[:T], want, ref.rotate_bound(q[:T].double(), want, turns, **kw)) == 0
+        ok(qo[:T], want, ref.rotate_bound(q[:T].double(), want, turns, **kw))
         new = ref.rotate(k[:T].double(), pos, turns, **kw)
         off = ref.rotate_bound(k[:T].double(), new, turns, **kw)
     else:
@@ -205,7 +211,8 @@ def test_append(pk, qs, kvs, Hq, Hkv, D, rot, P, interleaved, rows_first, pad, r
         page = int(host[b, p // P])
         want_k[page, :, p % P], bound[page, :, p % P] = new[t], off[t]
         want_v[page, :, p % P] = v[t].double()
-    assert ref.far(kc, want_k, bound) == 0 and torch.equal(vc.double(), want_v)
+    ok(kc, want_k, bound)
+    assert torch.equal(vc.double(), want_v)
     assert bool((qo[T:] == 3.0).all())
 
 
@@ -268,7 +275,7 @@ def run(pk, qs, kvs, Hq, Hkv, D, P, *, window=0, causal=True, rows_first=False, 
     s = scale if scale is not None else 1.0 / math.sqrt(D)
     want, bound = ref.attend(q[:T], kc, vc, table, q_start, kv_len, s, causal, window)
     assert bool((out[T:] == 5.0).all())
-    assert ref.far(out[:T], want, bound) == 0
+    ok(out[:T], want, bound)
     return out
 
 
@@ -406,7 +413,7 @@ def test_tables_out_of_range_are_brought_into_range(pk):
     kv_len = torch.tensor([-5, 10**9], dtype=torch.int32, device="cuda")
     pk.paged_attention(q, kc, vc, table, q_start, kv_len, out=out)
     want, bound = ref.attend(q, kc, vc, table, starts([3, 3]), torch.tensor([0, table.shape[1] * 16]), 0.125)
-    assert ref.far(out, want, bound) == 0
+    ok(out, want, bound)
     out.fill_(5.0)
     pk.paged_attention(q, kc, vc, table, torch.tensor([4, 2, 1], dtype=torch.int32, device="cuda"), kv_len, out=out)
     assert bool((out == 5.0).all())
@@ -427,7 +434,7 @@ def test_attention_strides_and_alignment(pk, qs, kvs, offset, pad):
     q_start, kv_len = starts(qs), torch.tensor(kvs, dtype=torch.int32, device="cuda")
     pk.paged_attention(q, kc, vc, table, q_start, kv_len, out=out)
     want, bound = ref.attend(q, kc, vc, table, q_start, kv_len, 0.125)
-    assert ref.far(out, want, bound) == 0
+    ok(out, want, bound)
 
 
 def test_offsets_past_32_bits(pk):
@@ -453,7 +460,7 @@ def test_offsets_past_32_bits(pk):
             assert torch.equal(kc[int(host[b, p // P]), :, p % P], k[t]) and torch.equal(vc[int(host[b, p // P]), :, p % P], v[t])
         out = pk.paged_attention(q, kc, vc, table, q_start, kv_len, max_q=max(qs))
         want, bound = ref.attend(q, kc, vc, table, q_start, kv_len, 1 / math.sqrt(D))
-        assert ref.far(out, want, bound) == 0
+        ok(out, want, bound)
         del kc, vc
 
 
@@ -500,7 +507,7 @@ def test_serving_run(pk, D, Hq, Hkv, P, interleaved):
             assert bool(((stored.double() - whole).abs() <= whole.abs() * 2.0**-8 + 2.0**-17).all())
             assert torch.equal(vc[dt[b][j // P].long(), :, j % P].double(), torch.cat(values[b]))
         want, bound = ref.attend(qr, kc, vc, dt, q_start, kv_len, 1 / math.sqrt(D))
-        assert ref.far(out, want, bound) == 0
+        ok(out, want, bound)
 
 
 def test_whole_prompt_equals_contiguous_attention(pk):
@@ -556,7 +563,7 @@ def test_steps_in_a_captured_graph(pk):
             eager = pk.paged_attention(qr, kcg, vcg, table, q_start, kv_len, max_q=n)
             assert torch.equal(replayed, eager) and torch.equal(kk, kcg)
             want, bound = ref.attend(qr, kcg, vcg, table, q_start, kv_len, 1 / math.sqrt(D))
-            assert ref.far(eager, want, bound) == 0
+            ok(eager, want, bound)
 
 
 def test_calls_on_several_streams(pk):
