@@ -103,9 +103,10 @@ template <int DP, bool PAGE16>
 __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
   using S = ChunkShape<DP>;
   using Tiles = TileLoader<DP, PAGE16, false>;
-  constexpr int CH = DP / 8, TB = S::TB, SL = S::SL, NI = Tiles::NI, DS = DP / 16, DB = DP / 32;
+  constexpr int CH = DP / 8, TB = S::TB, SL = S::SL, NI = Tiles::NI, DS = DP / 16, DB = DP / 32, RB = DP * 2;
+  constexpr int KO = DS < 8 ? DS : 8, VO = DB < 4 ? DB : 4;  // lane offsets; dims from 128 on lie 256 bytes further
   __shared__ __attribute__((aligned(1024))) uint8_t ring[S::LDS];
-  __shared__ uint16_t there_s[SL][PC_WAVES];
+  __shared__ __attribute__((aligned(8))) uint16_t there_s[SL][PC_WAVES];
   __shared__ int odd_s;
   const AttendArgs &g = d.a;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -140,12 +141,10 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
   // Q^T fragments: row lane % 32, dims 16 ds + 8 h + 0..7
   int lo, hi;
   bf16x8 qf[DS];
-  const int my = wrow + min(col, max(wrows, 1) - 1), my_row = min(my, all_rows - 1);
-  const int my_i = (int)g.group.div(my_row);
   {
-    key_range(g, s, my_i, lo, hi);
-    const uint16_t *qp = g.q.data + (int64_t)(s.q0 + my_i) * g.q.token +
-                         (it.hk * G + my_row - my_i * G) * g.q.head + 8 * h;
+    const int my = min(wrow + min(col, max(wrows, 1) - 1), all_rows - 1), i = (int)g.group.div(my);
+    key_range(g, s, i, lo, hi);
+    const uint16_t *qp = g.q.data + (int64_t)(s.q0 + i) * g.q.token + (it.hk * G + my - i * G) * g.q.head + 8 * h;
 #pragma unroll
     for (int ds = 0; ds < DS; ++ds) {
       att::u32x4 v = {0, 0, 0, 0};
@@ -156,8 +155,16 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
   }
   const float c2 = fabsf(g.c2);
 
-  auto issue = [&](int t) __attribute__((always_inline)) {
-    const int sl = t % SL;
+  // The lane's places in a K and a V tile; tile and row offsets are constants of the
+  // reads, since every slot of the rings has its own copy of the step.
+  uint32_t ko[KO], vo[VO];
+#pragma unroll
+  for (int ds = 0; ds < KO; ++ds) ko[ds] = (uint32_t)(col * RB + 16 * att::swz_k<CH>(2 * ds + h, col));
+#pragma unroll
+  for (int e = 0; e < VO; ++e)
+    vo[e] = (uint32_t)((4 * h + (gi >> 2)) * RB + 16 * ((4 * e + 2 * (grp & 1) + ((gi & 3) >> 1)) ^ att::swz_v<DP>(gi >> 2)) + 8 * (gi & 1));
+
+  auto issue = [&](int t, int sl) __attribute__((always_inline)) {
     tiles.issue(g, t, ring + sl * TB + wid * Tiles::BYTES, ring + (SL + sl) * TB + wid * Tiles::BYTES);
     const uint32_t is = tiles.there(t);  // by all lanes
     if (lane == 0) there_s[sl][wid] = (uint16_t)is;
@@ -171,50 +178,49 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
   float m_run = -INFINITY, l_run = 0.f;
   if (tid == 0) odd_s = 0;
 
-#pragma unroll
-  for (int t = 0; t < SL - 1; ++t) issue(t);
-#pragma unroll 1
-  for (int t = 0; t < nst; ++t) {
+  auto step = [&](auto slot, int t) __attribute__((always_inline)) {
+    constexpr int sl = decltype(slot)::value;
     vm_wait<2 * NI * (SL - 2)>();  // this wave's part of step t has landed
     lds_barrier();                 // and every wave's; nobody reads step t - 1 any more
-    const int sl = t % SL, key = kfirst + t * PC_STEP;
+    const int key = kfirst + t * PC_STEP;
     uint8_t *const ks = ring + sl * TB, *const vs = ring + (SL + sl) * TB;
-    const uint64_t there = (uint64_t)there_s[sl][0] | (uint64_t)there_s[sl][1] << 16 | (uint64_t)there_s[sl][2] << 32 |
-                           (uint64_t)there_s[sl][3] << 48;
-    const uint32_t there_lo = uniform((int)(uint32_t)there), there_hi = uniform((int)(uint32_t)(there >> 32));
-    issue(t + SL - 1);
-    const bool any = wrows > 0 && key < hi_any && key + PC_STEP > lo_any && (there_lo | there_hi) != 0;
-    const bool whole = (there_lo & there_hi) == 0xFFFFFFFFu;
+    const att::u32x2 there_w = *reinterpret_cast<const att::u32x2 *>(there_s[sl]);
+    issue(t + SL - 1, (sl + SL - 1) % SL);
+    const uint32_t there[2] = {(uint32_t)uniform((int)there_w[0]), (uint32_t)uniform((int)there_w[1])};
+    const bool any = wrows > 0 && key < hi_any && key + PC_STEP > lo_any && (there[0] | there[1]) != 0;
+    const bool whole = (there[0] & there[1]) == 0xFFFFFFFFu;
     const bool masked = key < lo_all || key + PC_STEP > hi_all || !whole;
     // the same for every wave: whether some row of the item has a hidden key in this step
     const bool mixed = key < t1 || key + PC_STEP > t0 || !whole;
 
     bf16x8 pf[4];
-    uint32_t hid = 0;  // hidden keys of this lane's 32
+    uint32_t seen[2] = {~0u, ~0u};  // keys 32 kb + 4 h + b, bit b of word kb
     if (any) {
       f32x16 sc[2];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
+      for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[kb][i] = 0.f;
-        const int row = 32 * kb + col;
 #pragma unroll
-        for (int ds = 0; ds < DS; ++ds) {
-          const att::u32x4 kv = *reinterpret_cast<const att::u32x4 *>(ks + row * DP * 2 + 16 * att::swz_k<CH>(2 * ds + h, row));
+      for (int ds = 0; ds < DS; ++ds)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          const att::u32x4 kv = *reinterpret_cast<const att::u32x4 *>(ks + ko[ds % KO] + 256 * (ds / KO) + 32 * kb * RB);
           sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kv), qf[ds], sc[kb], 0, 0, 0);
         }
-      }
       if (masked) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < 2; ++kb) {
+          // keys [lo, hi) of this half as bits, those on pages that are not there taken out
+          const int from = min(max(lo - key - 32 * kb, 0), 32), to = min(max(hi - key - 32 * kb, 0), 32);
+          const uint32_t up = to < 32 ? (1u << to) - 1 : ~0u, down = from < 32 ? ~0u << from : 0u;
+          seen[kb] = (up & down & there[kb]) >> (4 * h);
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const int kk = 8 * (i >> 2) + 4 * h + (i & 3), k = key + 32 * kb + kk;
-            if (k < lo || k >= hi || !((kb ? there_hi : there_lo) >> kk & 1)) {
-              sc[kb][i] = -INFINITY;
-              hid |= 1u << (16 * kb + i);
-            }
+            const int on = __builtin_amdgcn_sbfe((int)seen[kb], 8 * (i >> 2) + (i & 3), 1);  // all bits or none
+            sc[kb][i] = __uint_as_float(((uint32_t)on & __float_as_uint(sc[kb][i])) | (~(uint32_t)on & 0xFF800000u));
           }
+        }
       }
       float top = sc[0][0];
 #pragma unroll
@@ -253,14 +259,14 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
     // signs) at 2^127 and the keys that a row sees at 2^127: sums overflow to what the row sees.
     int pass = 3;
     if (mixed) {
-      bool odd = false;
+      pk_u16x2 most = {0, 0};
 #pragma unroll
       for (int i = 0; i < TB / (16 * PC_THREADS); ++i) {
         const att::u32x4 w = *reinterpret_cast<const att::u32x4 *>(vs + 16 * (tid + i * PC_THREADS));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) odd |= word_not_finite(w[e]);
+        for (int e = 0; e < 4; ++e) most = exponents(most, w[e]);
       }
-      if (__any(odd) && lane == 0) odd_s = 1;
+      if (__any(not_finite(most)) && lane == 0) odd_s = 1;
       lds_barrier();
       if (uniform(odd_s)) pass = 0;
     }
@@ -279,13 +285,15 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
         }
         if (tid == 0) odd_s = 0;
         if (pass > 0) {
+          asm volatile("" : "+v"(seen[0]), "+v"(seen[1]));  // computed here, not before every step
 #pragma unroll
           for (int st = 0; st < 4; ++st) {
             att::u32x4 w;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const uint32_t two = hid >> (8 * st + 2 * i);
-              w[i] = (two & 1 ? 0u : 0x7F00u) | (two & 2 ? 0u : 0x7F000000u);
+              const int j = 8 * (st & 1) + 2 * i;
+              const uint32_t two = seen[st >> 1] >> (8 * (j >> 2) + (j & 3));
+              w[i] = (two & 1 ? 0x7F00u : 0u) | (two & 2 ? 0x7F000000u : 0u);
             }
             pf[st] = __builtin_bit_cast(bf16x8, w);
           }
@@ -299,17 +307,25 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
           for (int e = 0; e < DB; ++e) {
             i16x4 hv[2];
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const int kr = st * 16 + 8 * r + 4 * h + (gi >> 2), dd = e * 32 + 16 * (grp & 1) + 4 * (gi & 3);
+            for (int r = 0; r < 2; ++r)
               hv[r] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                  (att::lds_i16x4 *)(vs + kr * DP * 2 + 16 * ((dd >> 3) ^ att::swz_v<DP>(kr)) + 2 * (dd & 7)));
-            }
+                  (att::lds_i16x4 *)(vs + vo[e % VO] + 256 * (e / VO) + (st * 16 + 8 * r) * RB));
             const bf16x8 va = __builtin_bit_cast(bf16x8, __builtin_shufflevector(hv[0], hv[1], 0, 1, 2, 3, 4, 5, 6, 7));
             acc[e] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pf[st], acc[e], 0, 0, 0);
           }
       }
       if (pass >= 2) break;
     }
+  };
+
+#pragma unroll
+  for (int t = 0; t < SL - 1; ++t) issue(t, t);
+#pragma unroll 1
+  for (int t = 0; t < nst; t += SL) {
+    step(std::integral_constant<int, 0>{}, t);
+    if (t + 1 < nst) step(std::integral_constant<int, 1>{}, t + 1);
+    if constexpr (SL == 3)
+      if (t + 2 < nst) step(std::integral_constant<int, 2>{}, t + 2);
   }
   vm_wait<0>();
   l_run = xor32_sum(l_run);

@@ -306,14 +306,14 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
           // 2^127 and the keys that a row sees at 2^127: sums overflow to what the row sees.
           bool apart = false;
           if (masked) {
-            bool odd = false;
+            pk_u16x2 most = {0, 0};
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
               const att::u32x4 w = *reinterpret_cast<const att::u32x4 *>(vs + i * 1024 + 16 * lane);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) odd |= word_not_finite(w[e]);
+              for (int e = 0; e < 4; ++e) most = exponents(most, w[e]);
             }
-            apart = __any(odd);
+            apart = __any(not_finite(most));
           }
 #pragma unroll 1
           for (int pass = apart ? 0 : 3;; ++pass) {
@@ -330,7 +330,8 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
               if (pass > 0) {
 #pragma unroll
                 for (int m = 0; m < MT; ++m) {
-                  const uint32_t h = hid[m];
+                  uint32_t h = hid[m];
+                  asm volatile("" : "+v"(h));  // computed here, not before every step
                   phi[m] = __builtin_bit_cast(i16x4, (att::u32x2{(h & 1 ? 0u : 0x7F00u) | (h & 2 ? 0u : 0x7F000000u),
                                                                  (h & 4 ? 0u : 0x7F00u) | (h & 8 ? 0u : 0x7F000000u)}));
                   plo[m] = i16x4{0, 0, 0, 0};

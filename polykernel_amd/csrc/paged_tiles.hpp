@@ -139,10 +139,12 @@ struct TileLoader {
   }
 };
 
-// Whether either half of a word is no number or infinite.
-__device__ __forceinline__ bool word_not_finite(uint32_t w) {
-  return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
+// The largest exponent fields seen in the halves of words, and whether one is that of an
+// infinity or no number.
+__device__ __forceinline__ pk_u16x2 exponents(pk_u16x2 most, uint32_t w) {
+  return __builtin_elementwise_max(most, __builtin_bit_cast(pk_u16x2, w & 0x7F807F80u));
 }
+__device__ __forceinline__ bool not_finite(pk_u16x2 most) { return most.x >= 0x7F80 || most.y >= 0x7F80; }
 
 // A value (low half of w) for the passes over a tile with values that are no numbers: 0
 // keeps the finite ones, 1 and 2 hold 2^127 and -2^127 where it is +inf and -inf, both
