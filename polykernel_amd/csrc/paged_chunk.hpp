@@ -6,8 +6,11 @@
 // O^T = V^T P^T run on v_mfma_f32_32x32x16_bf16 as in the contiguous flash kernel: a lane
 // owns one row and half of the keys, so P never leaves its registers.  P is rounded to
 // bf16 once (half a step, 2^-8 of a weight, its sum kept in fp32): the second product
-// of a low half would be a third of all matrix work.  Two workgroups share a CU, so that
-// one's softmax runs beside the other's products.
+// of a low half would be a third of all matrix work.
+//
+// Step t + 1's scores are computed while step t's exponentials are, in one run of
+// instructions without a branch (two waves of two workgroups on a SIMD fall into step
+// otherwise, and both wait for the matrix unit and then both for the exponentials).
 //
 // Items of one key head run next to each other on one XCD and share its L2; a sequence's
 // last rows, which see the most keys, come first.  Few items are also cut into `splits`
@@ -122,7 +125,7 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
   const int rows = min(PC_ROWS, all_rows - row0);
   const int wrow = row0 + 32 * wid, wrows = min(32, all_rows - wrow);  // this wave's (may be none)
 
-  // the item's keys, and the keys that all and any of this wave's rows see
+  // the item's keys, and those that all of this wave's rows see
   int lo_first, hi_last, t0, t1;
   key_range(g, s, (int)g.group.div(row0), lo_first, t0);
   key_range(g, s, (int)g.group.div(row0 + rows - 1), t1, hi_last);
@@ -132,11 +135,9 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
   const int kfirst = klo + s0 * PC_STEP;
   Tiles tiles(g);
   tiles.begin(g, it.b, it.hk, kfirst + wid * PT_KEYS, nst, hi_last);
-  int lo_any = 0, hi_all = 0, lo_all = 0, hi_any = 0;
-  if (wrows > 0) {
-    key_range(g, s, (int)g.group.div(wrow), lo_any, hi_all);
-    key_range(g, s, (int)g.group.div(wrow + wrows - 1), lo_all, hi_any);
-  }
+  int lo_all, hi_all, t2, t3;
+  key_range(g, s, (int)g.group.div(min(wrow, all_rows - 1)), t2, hi_all);
+  key_range(g, s, (int)g.group.div(min(wrow + 31, all_rows - 1)), lo_all, t3);
 
   // Q^T fragments: row lane % 32, dims 16 ds + 8 h + 0..7
   int lo, hi;
@@ -164,162 +165,185 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
   for (int e = 0; e < VO; ++e)
     vo[e] = (uint32_t)((4 * h + (gi >> 2)) * RB + 16 * ((4 * e + 2 * (grp & 1) + ((gi & 3) >> 1)) ^ att::swz_v<DP>(gi >> 2)) + 8 * (gi & 1));
 
-  auto issue = [&](int t, int sl) __attribute__((always_inline)) {
-    tiles.issue(g, t, ring + sl * TB + wid * Tiles::BYTES, ring + (SL + sl) * TB + wid * Tiles::BYTES);
+  // K of step t and V of step t lie in slot t % SL of their rings.  Step t's iteration reads K
+  // of step t + 1 and V of step t, and loads K of step t + SL (K of step t has been read) and
+  // V of step t + SL - 1 (V of step t - 1 has).
+  auto issue_k = [&](int t, int sl) __attribute__((always_inline)) {
+    tiles.issue_k(g, t, ring + sl * TB + wid * Tiles::BYTES);
     const uint32_t is = tiles.there(t);  // by all lanes
     if (lane == 0) there_s[sl][wid] = (uint16_t)is;
   };
+  auto issue_v = [&](int t, int sl) __attribute__((always_inline)) {
+    tiles.issue_v(g, t, ring + (SL + sl) * TB + wid * Tiles::BYTES);
+  };
 
-  f32x16 acc[DB];
+  f32x16 acc[DB], sc[2];
 #pragma unroll
   for (int e = 0; e < DB; ++e)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[e][i] = 0.f;
-  float m_run = -INFINITY, l_run = 0.f;
-  if (tid == 0) odd_s = 0;
+  float m_run = -INFINITY, l_run = 0.f, top = -INFINITY;  // top: row maximum of sc
+  bool whole = true;                   // the keys of the step in sc are all on pages that are there
+  int odd_first = nst, odd_last = -1;  // steps whose values were not all finite where a row has a hidden key
+  if (tid == 0) odd_s = -1;
 
-  auto step = [&](auto slot, int t) __attribute__((always_inline)) {
-    constexpr int sl = decltype(slot)::value;
-    vm_wait<2 * NI * (SL - 2)>();  // this wave's part of step t has landed
-    lds_barrier();                 // and every wave's; nobody reads step t - 1 any more
+  // fragment i of the 2 DS of a K tile: head dims 16 (i / 2) + ..., keys 32 (i % 2) + ...
+  auto k_fragment = [&](int sl, int i) __attribute__((always_inline)) {
+    const int ds = i >> 1;
+    return __builtin_bit_cast(bf16x8, *reinterpret_cast<const att::u32x4 *>(ring + sl * TB + ko[ds % KO] + 256 * (ds / KO) +
+                                                                            32 * (i & 1) * RB));
+  };
+  // fragment i of the 4 DB of a V tile: keys 16 (i / DB) + ..., head dims 32 (i % DB) + ...
+  auto v_fragment = [&](int sl, int i) __attribute__((always_inline)) {
+    const int st = i / DB, e = i % DB;
+    i16x4 hv[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+      hv[r] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (att::lds_i16x4 *)(ring + (SL + sl) * TB + vo[e % VO] + 256 * (e / VO) + (st * 16 + 8 * r) * RB));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(hv[0], hv[1], 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  // Scores of the step in K slot sl, and beside product i the work of `beside(i)`.  Fragments
+  // are read AHEAD products before they are used, and the order is kept as written.
+  constexpr int AHEAD = 4, NA = 2 * DS, NB = 4 * DB;
+  auto scores = [&](int sl, f32x16 (&x)[2], auto beside) __attribute__((always_inline)) {
+    bf16x8 f[NA];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) f[i] = k_fragment(sl, i);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+      if (i < 2) x[i] = f32x16{};
+      x[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[i], qf[i >> 1], x[i & 1], 0, 0, 0);
+      if (i + AHEAD < NA) f[i + AHEAD] = k_fragment(sl, i + AHEAD);
+      beside(i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto maximum = [&](const f32x16 (&x)[2]) __attribute__((always_inline)) {
+    float m = x[0][0];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) m = fmaxf(m, x[kb][i]);
+    return xor32_max(m);
+  };
+  // hides what this wave's rows do not see of step t, whose scores are in sc (K slot sl)
+  auto mask = [&](int t, int sl) __attribute__((always_inline)) {
+    const att::u32x2 w = *reinterpret_cast<const att::u32x2 *>(there_s[sl]);
+    const uint32_t there[2] = {(uint32_t)uniform((int)w[0]), (uint32_t)uniform((int)w[1])};
     const int key = kfirst + t * PC_STEP;
-    uint8_t *const ks = ring + sl * TB, *const vs = ring + (SL + sl) * TB;
-    const att::u32x2 there_w = *reinterpret_cast<const att::u32x2 *>(there_s[sl]);
-    issue(t + SL - 1, (sl + SL - 1) % SL);
-    const uint32_t there[2] = {(uint32_t)uniform((int)there_w[0]), (uint32_t)uniform((int)there_w[1])};
-    const bool any = wrows > 0 && key < hi_any && key + PC_STEP > lo_any && (there[0] | there[1]) != 0;
-    const bool whole = (there[0] & there[1]) == 0xFFFFFFFFu;
-    const bool masked = key < lo_all || key + PC_STEP > hi_all || !whole;
-    // the same for every wave: whether some row of the item has a hidden key in this step
-    const bool mixed = key < t1 || key + PC_STEP > t0 || !whole;
-
-    bf16x8 pf[4];
-    uint32_t seen[2] = {~0u, ~0u};  // keys 32 kb + 4 h + b, bit b of word kb
-    if (any) {
-      f32x16 sc[2];
+    whole = (there[0] & there[1]) == 0xFFFFFFFFu;
+    if (key < lo_all || key + PC_STEP > hi_all || !whole) {
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+      for (int kb = 0; kb < 2; ++kb) {
+        // keys [lo, hi) of this half as bits, those on pages that are not there taken out
+        const int from = min(max(lo - key - 32 * kb, 0), 32), to = min(max(hi - key - 32 * kb, 0), 32);
+        const uint32_t up = to < 32 ? (1u << to) - 1 : ~0u, down = from < 32 ? ~0u << from : 0u;
+        const uint32_t seen = (up & down & there[kb]) >> (4 * h);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sc[kb][i] = 0.f;
-#pragma unroll
-      for (int ds = 0; ds < DS; ++ds)
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          const att::u32x4 kv = *reinterpret_cast<const att::u32x4 *>(ks + ko[ds % KO] + 256 * (ds / KO) + 32 * kb * RB);
-          sc[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, kv), qf[ds], sc[kb], 0, 0, 0);
-        }
-      if (masked) {
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-          // keys [lo, hi) of this half as bits, those on pages that are not there taken out
-          const int from = min(max(lo - key - 32 * kb, 0), 32), to = min(max(hi - key - 32 * kb, 0), 32);
-          const uint32_t up = to < 32 ? (1u << to) - 1 : ~0u, down = from < 32 ? ~0u << from : 0u;
-          seen[kb] = (up & down & there[kb]) >> (4 * h);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int on = __builtin_amdgcn_sbfe((int)seen[kb], 8 * (i >> 2) + (i & 3), 1);  // all bits or none
-            sc[kb][i] = __uint_as_float(((uint32_t)on & __float_as_uint(sc[kb][i])) | (~(uint32_t)on & 0xFF800000u));
-          }
+        for (int i = 0; i < 16; ++i) {
+          const int on = __builtin_amdgcn_sbfe((int)seen, 8 * (i >> 2) + (i & 3), 1);  // all bits or none
+          sc[kb][i] = __uint_as_float(((uint32_t)on & __float_as_uint(sc[kb][i])) | (~(uint32_t)on & 0xFF800000u));
         }
       }
-      float top = sc[0][0];
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[kb][i]);
-      top = xor32_max(top);
-      // the maximum in the exponent follows once it is 2^8 behind
-      if (__any((top - m_run) * c2 > 8.f)) {
-        const float m_new = fmaxf(m_run, top);
-        const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - m_new) * c2);
-        m_run = m_new;
-        l_run *= alpha;
-#pragma unroll
-        for (int e = 0; e < DB; ++e) acc[e] *= alpha;
-      }
-      const float mc = m_run == -INFINITY ? 0.f : m_run * c2;
-      float sum = 0.f;
-#pragma unroll
-      for (int st = 0; st < 4; ++st) {
-        att::u32x4 w;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int kb = st >> 1, j = 8 * (st & 1) + 2 * i;
-          const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[kb][j], c2, -mc));
-          const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[kb][j + 1], c2, -mc));
-          sum += p0 + p1;
-          w[i] = pack_bf(p0, p1);
-        }
-        pf[st] = __builtin_bit_cast(bf16x8, w);
-      }
-      l_run += sum;
-    }
-    // A hidden key's value that is no number must not meet its zero weight: the workgroup
-    // multiplies such a step with those values at zero, then with each infinity (a NaN as both
-    // signs) at 2^127 and the keys that a row sees at 2^127: sums overflow to what the row sees.
-    int pass = 3;
-    if (mixed) {
-      pk_u16x2 most = {0, 0};
-#pragma unroll
-      for (int i = 0; i < TB / (16 * PC_THREADS); ++i) {
-        const att::u32x4 w = *reinterpret_cast<const att::u32x4 *>(vs + 16 * (tid + i * PC_THREADS));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) most = exponents(most, w[e]);
-      }
-      if (__any(not_finite(most)) && lane == 0) odd_s = 1;
-      lds_barrier();
-      if (uniform(odd_s)) pass = 0;
-    }
-#pragma unroll 1
-    for (;; ++pass) {
-      if (pass < 3) {  // the step's values as they were are kept in the slot of its keys
-        lds_barrier();
-#pragma unroll 1
-        for (int i = 0; i < TB / (16 * PC_THREADS); ++i) {
-          const int x = 16 * (tid + i * PC_THREADS);
-          att::u32x4 w = *reinterpret_cast<const att::u32x4 *>((pass ? ks : vs) + x);
-          if (pass == 0) *reinterpret_cast<att::u32x4 *>(ks + x) = w;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = apart_half(w[e], pass) | apart_half(w[e] >> 16, pass) << 16;
-          *reinterpret_cast<att::u32x4 *>(vs + x) = w;
-        }
-        if (tid == 0) odd_s = 0;
-        if (pass > 0) {
-          asm volatile("" : "+v"(seen[0]), "+v"(seen[1]));  // computed here, not before every step
-#pragma unroll
-          for (int st = 0; st < 4; ++st) {
-            att::u32x4 w;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int j = 8 * (st & 1) + 2 * i;
-              const uint32_t two = seen[st >> 1] >> (8 * (j >> 2) + (j & 3));
-              w[i] = (two & 1 ? 0x7F00u : 0u) | (two & 2 ? 0x7F000000u : 0u);
-            }
-            pf[st] = __builtin_bit_cast(bf16x8, w);
-          }
-        }
-        lds_barrier();
-      }
-      if (any) {
-#pragma unroll
-        for (int st = 0; st < 4; ++st)
-#pragma unroll
-          for (int e = 0; e < DB; ++e) {
-            i16x4 hv[2];
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
-              hv[r] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                  (att::lds_i16x4 *)(vs + vo[e % VO] + 256 * (e / VO) + (st * 16 + 8 * r) * RB));
-            const bf16x8 va = __builtin_bit_cast(bf16x8, __builtin_shufflevector(hv[0], hv[1], 0, 1, 2, 3, 4, 5, 6, 7));
-            acc[e] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pf[st], acc[e], 0, 0, 0);
-          }
-      }
-      if (pass >= 2) break;
+      top = maximum(sc);
     }
   };
 
+  auto step = [&](auto slot, int t) __attribute__((always_inline)) {
+    constexpr int sl = decltype(slot)::value, next = (sl + 1) % SL;
+    vm_wait<2 * NI * (SL - 2)>();  // this wave's part of K of step t + 1 and V of step t has landed
+    lds_barrier();                 // and every wave's; nobody reads what the next loads overwrite
+    uint8_t *const vs = ring + (SL + sl) * TB;
+    const int key = kfirst + t * PC_STEP;
+    // the same for every wave: whether some row of the item has a hidden key in this step
+    const bool mixed = key < t1 || key + PC_STEP > t0 || !whole;
+    issue_k(t + SL, sl);
+    issue_v(t + SL - 1, (sl + SL - 1) % SL);
+
+    // the maximum in the exponent follows once it is 2^8 behind
+    if (__any((top - m_run) * c2 > 8.f)) {
+      const float m_new = fmaxf(m_run, top);
+      const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - m_new) * c2);
+      m_run = m_new;
+      l_run *= alpha;
 #pragma unroll
-  for (int t = 0; t < SL - 1; ++t) issue(t, t);
+      for (int e = 0; e < DB; ++e) acc[e] *= alpha;
+    }
+    const float mc = m_run == -INFINITY ? 0.f : m_run * c2;
+    f32x16 nx[2];
+    att::u32x4 pw[4];
+    float sum = 0.f;
+    scores(next, nx, [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+      for (int n = i * 16 / NA; n < (i + 1) * 16 / NA; ++n) {  // two of the 32 scores
+        const int kb = n >> 3, j = 2 * (n & 7);
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[kb][j], c2, -mc));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[kb][j + 1], c2, -mc));
+        sum += p0 + p1;
+        uint32_t two = pack_bf(p0, p1);
+        asm volatile("" : "+v"(two));  // here, not where it is used first
+        pw[n >> 2][n & 3] = two;
+      }
+    });
+    l_run += sum;
+
+    if (mixed) {
+      pk_u16x2 most = {0, 0};
+#pragma unroll 1
+      for (int x = 16 * tid; x < TB; x += 16 * PC_THREADS) {
+        const att::u32x4 w = *reinterpret_cast<const att::u32x4 *>(vs + x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = exponents(most, w[e]);
+      }
+      if (__any(not_finite(most)) && lane == 0) odd_s = t;
+      lds_barrier();
+      if (uniform(odd_s) == t) {
+        odd_first = min(odd_first, t);
+        odd_last = t;
+#pragma unroll 1
+        for (int x = 16 * tid; x < TB; x += 16 * PC_THREADS) {
+          att::u32x4 *at = reinterpret_cast<att::u32x4 *>(vs + x), w = *at;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = finite(w[e]);
+          *at = w;
+        }
+        lds_barrier();
+      }
+    }
+    {
+      bf16x8 f[NB];
+      top = nx[0][0];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) f[i] = v_fragment(sl, i);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        acc[i % DB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[i], __builtin_bit_cast(bf16x8, pw[i / DB]), acc[i % DB], 0, 0, 0);
+        if (i + AHEAD < NB) f[i + AHEAD] = v_fragment(sl, i + AHEAD);
+#pragma unroll
+        for (int n = i * 32 / NB; n < (i + 1) * 32 / NB; ++n) top = fmaxf(top, nx[n >> 4][n & 15]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      top = xor32_max(top);
+    }
+    sc[0] = nx[0];
+    sc[1] = nx[1];
+    mask(t + 1, next);
+  };
+
+  issue_k(0, 0);
+#pragma unroll
+  for (int t = 0; t < SL - 1; ++t) {
+    issue_k(t + 1, t + 1);
+    issue_v(t, t);
+  }
+  vm_wait<2 * NI * (SL - 1)>();
+  lds_barrier();
+  scores(0, sc, [](int) {});
+  top = maximum(sc);
+  mask(0, 0);
 #pragma unroll 1
   for (int t = 0; t < nst; t += SL) {
     step(std::integral_constant<int, 0>{}, t);
@@ -329,6 +353,20 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
   }
   vm_wait<0>();
   l_run = xor32_sum(l_run);
+  for (int k = kfirst + odd_first * PC_STEP; k < min(hi_last, kfirst + (odd_last + 1) * PC_STEP); ++k) {
+    const uint16_t *vr = value_row(g, it.b, it.hk, k);
+    if (!vr || k < lo || k >= hi) continue;
+#pragma unroll
+    for (int e = 0; e < DB; ++e)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (32 * e + 8 * j + 4 * h < D) {
+          f32x4 x = {acc[e][4 * j], acc[e][4 * j + 1], acc[e][4 * j + 2], acc[e][4 * j + 3]};
+          add_not_finite(vr + 32 * e + 8 * j + 4 * h, x);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[e][4 * j + i] = x[i];
+        }
+  }
 
   if (d.splits > 1) {
     // this split's state of the rows

@@ -213,7 +213,8 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
     const float c2 = fabsf(g.c2);
 
     auto issue = [&](int t) __attribute__((always_inline)) {
-      tiles.issue(g, t, mine + (t % SL) * TB, mine + (SL + t % SL) * TB);
+      tiles.issue_k(g, t, mine + (t % SL) * TB);
+      tiles.issue_v(g, t, mine + (SL + t % SL) * TB);
     };
     float m_run[MT], l_run[MT];
     f32x4 acc[MT][DB];
@@ -231,6 +232,7 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
       issue(t);
       there |= (uint64_t)tiles.there(t) << (16 * t);
     }
+    int odd_first = nst, odd_last = -1;  // tiles whose values were not all finite where a row has a hidden key
 #pragma unroll 1
     for (int t = 0; t < nst; ++t) {
       {
@@ -262,19 +264,14 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
         }
         vm_wait<2 * NI * (SL - 1)>();
         if (any) {
-          uint32_t hid[MT];  // hidden keys of this lane's four
           i16x4 phi[MT], plo[MT];
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
-            hid[m] = 0;
             if (masked) {
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const int kk = 4 * grp + i;
-                if (key + kk < lo[m] || key + kk >= hi[m] || !(here >> kk & 1)) {
-                  sc[m][i] = -INFINITY;
-                  hid[m] |= 1u << i;
-                }
+                if (key + kk < lo[m] || key + kk >= hi[m] || !(here >> kk & 1)) sc[m][i] = -INFINITY;
               }
             }
             float top = fmaxf(fmaxf(sc[m][0], sc[m][1]), fmaxf(sc[m][2], sc[m][3]));
@@ -301,55 +298,36 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
             plo[m] = __builtin_bit_cast(i16x4, (att::u32x2{pack_bf(p[0] - lo_bf(h0), p[1] - hi_bf(h0)),
                                                            pack_bf(p[2] - lo_bf(h1), p[3] - hi_bf(h1))}));
           }
-          // A hidden key's value that is no number must not meet its zero weight: such a tile is
-          // multiplied with those values at zero, then with each infinity (a NaN as both signs) at
-          // 2^127 and the keys that a row sees at 2^127: sums overflow to what the row sees.
-          bool apart = false;
           if (masked) {
             pk_u16x2 most = {0, 0};
-#pragma unroll
+#pragma unroll 1
             for (int i = 0; i < NI; ++i) {
               const att::u32x4 w = *reinterpret_cast<const att::u32x4 *>(vs + i * 1024 + 16 * lane);
 #pragma unroll
               for (int e = 0; e < 4; ++e) most = exponents(most, w[e]);
             }
-            apart = __any(not_finite(most));
-          }
-#pragma unroll 1
-          for (int pass = apart ? 0 : 3;; ++pass) {
-            if (pass < 3) {  // the tile as it was is kept in the slot of its keys
+            if (__any(not_finite(most))) {
+              odd_first = min(odd_first, t);
+              odd_last = t;
 #pragma unroll 1
               for (int i = 0; i < NI; ++i) {
-                const int x = i * 1024 + 16 * lane;
-                att::u32x4 w = *reinterpret_cast<const att::u32x4 *>((pass ? ks : vs) + x);
-                if (pass == 0) *reinterpret_cast<att::u32x4 *>(ks + x) = w;
+                att::u32x4 *at = reinterpret_cast<att::u32x4 *>(vs + i * 1024 + 16 * lane), w = *at;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = apart_half(w[e], pass) | apart_half(w[e] >> 16, pass) << 16;
-                *reinterpret_cast<att::u32x4 *>(vs + x) = w;
-              }
-              if (pass > 0) {
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                  uint32_t h = hid[m];
-                  asm volatile("" : "+v"(h));  // computed here, not before every step
-                  phi[m] = __builtin_bit_cast(i16x4, (att::u32x2{(h & 1 ? 0u : 0x7F00u) | (h & 2 ? 0u : 0x7F000000u),
-                                                                 (h & 4 ? 0u : 0x7F00u) | (h & 8 ? 0u : 0x7F000000u)}));
-                  plo[m] = i16x4{0, 0, 0, 0};
-                }
+                for (int e = 0; e < 4; ++e) w[e] = finite(w[e]);
+                *at = w;
               }
             }
+          }
 #pragma unroll
-            for (int e = 0; e < DB; ++e) {
-              const int key_r = 4 * grp + (col >> 2), c = 2 * e + (col & 3) / 2;
-              const i16x4 vf = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                  (att::lds_i16x4 *)(vs + key_r * DP * 2 + 16 * (c ^ att::swz_v<DP>(key_r)) + 8 * (col & 1)));
+          for (int e = 0; e < DB; ++e) {
+            const int key_r = 4 * grp + (col >> 2), c = 2 * e + (col & 3) / 2;
+            const i16x4 vf = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (att::lds_i16x4 *)(vs + key_r * DP * 2 + 16 * (c ^ att::swz_v<DP>(key_r)) + 8 * (col & 1)));
 #pragma unroll
-              for (int m = 0; m < MT; ++m) {
-                acc[m][e] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vf, phi[m], acc[m][e], 0, 0, 0);
-                acc[m][e] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vf, plo[m], acc[m][e], 0, 0, 0);
-              }
+            for (int m = 0; m < MT; ++m) {
+              acc[m][e] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vf, phi[m], acc[m][e], 0, 0, 0);
+              acc[m][e] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vf, plo[m], acc[m][e], 0, 0, 0);
             }
-            if (pass >= 2) break;
           }
         }
         lgkm_wait0();  // the slot's reads are done
@@ -358,6 +336,17 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
       }
     }
     vm_wait<0>();
+    for (int t = odd_first; t <= odd_last; ++t)
+      for (int k = key0 + t * PD_STEP; k < min(hi_any, key0 + t * PD_STEP + PD_TILE); ++k) {
+        const uint16_t *vr = value_row(g, b, hk, k);
+        if (!vr) continue;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+          if (k >= lo[m] && k < hi[m])
+#pragma unroll
+            for (int e = 0; e < DB; ++e)
+              if (16 * e + 4 * grp < D) add_not_finite(vr + 16 * e + 4 * grp, acc[m][e]);
+      }
 
     // ---- the waves' states, added in wave order
 #pragma unroll

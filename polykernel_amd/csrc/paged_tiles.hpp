@@ -74,7 +74,8 @@ struct TileLoader {
   static constexpr int BATCH = PAGE16 ? 64 : 4;
   uint32_t kvo[NI], vvo[NI];
   const uint16_t *kbase, *vbase;
-  int b, key0, count, hi, pages;
+  int b, key0, count, hi;
+  int kpages, vpages;  // of the batch that the last K and the last V tile is in
 
   // lane's part of instruction i: row i RPI + lane / CH, chunk by its swizzle
   __device__ __forceinline__ static int row_of(int i) { return i * RPI + (int)(threadIdx.x & 63) / CH; }
@@ -88,54 +89,55 @@ struct TileLoader {
       vvo[i] = 8 * v_chunk(i) < g.cache.dim ? (uint32_t)(row_of(i) * (int)g.cache.v_row * 2 + 16 * v_chunk(i)) : 0x80000000u;
     }
   }
-  __device__ __forceinline__ void look_up(const AttendArgs &g, int t) {
+  __device__ __forceinline__ int look_up(const AttendArgs &g, int t) const {
     const int lane = threadIdx.x & 63;
     const int key = key0 + (PAGE16 ? (t + lane) * PT_STEP : (t + (lane >> 4)) * PT_STEP + (lane & 15));
-    pages = key < hi ? page_of(g.batch, g.cache, b, key) : -1;
+    return key < hi ? page_of(g.batch, g.cache, b, key) : -1;
   }
   __device__ __forceinline__ void begin(const AttendArgs &g, int b_, int hk, int key0_, int count_, int hi_) {
     b = b_, key0 = key0_, count = count_, hi = hi_;
     kbase = g.cache.k + hk * g.cache.k_head;
     vbase = g.cache.v + hk * g.cache.v_head;
-    look_up(g, 0);
+    kpages = vpages = look_up(g, 0);
   }
-  // Tiles in order from 0; tiles from `count` on load nothing (as many instructions, of no length).
-  __device__ __forceinline__ void issue(const AttendArgs &g, int t, uint8_t *ks, uint8_t *vs) {
-    if (t % BATCH == 0 && t > 0 && t < count) look_up(g, t);
+  // Tiles of K, and of V, in order from 0; tiles from `count` on load nothing (as many
+  // instructions, of no length).
+  __device__ __forceinline__ void issue_k(const AttendArgs &g, int t, uint8_t *to) {
+    if (t % BATCH == 0 && t > 0 && t < count) kpages = look_up(g, t);
+    load(g, t, kpages, kbase, g.cache.k_page, g.cache.k_row, kvo, [](int i) { return k_chunk(i); }, to);
+  }
+  __device__ __forceinline__ void issue_v(const AttendArgs &g, int t, uint8_t *to) {
+    if (t % BATCH == 0 && t > 0 && t < count) vpages = look_up(g, t);
+    load(g, t, vpages, vbase, g.cache.v_page, g.cache.v_row, vvo, [](int i) { return v_chunk(i); }, to);
+  }
+  template <typename Chunk>
+  __device__ __forceinline__ void load(const AttendArgs &g, int t, int pages, const uint16_t *base, int64_t page_stride,
+                                       int64_t row_stride, const uint32_t (&offset)[NI], Chunk chunk, uint8_t *to) {
     const int key = key0 + t * PT_STEP, left = t < count ? hi - key : 0;
     if constexpr (PAGE16) {
       const int page = __builtin_amdgcn_readlane(pages, t % BATCH), n = page < 0 ? 0 : min(PT_KEYS, left);
       const int row = n > 0 ? key - (int)(g.cache.page.div(key) * g.cache.page.d) : 0;
-      const int64_t pg = n > 0 ? page : 0;
-      const pk_u32x4 kr = rsrc_words(kbase + pg * g.cache.k_page + row * g.cache.k_row,
-                                     n > 0 ? (uint32_t)(((n - 1) * (int)g.cache.k_row + g.cache.dim) * 2) : 0u);
-      const pk_u32x4 vr = rsrc_words(vbase + pg * g.cache.v_page + row * g.cache.v_row,
-                                     n > 0 ? (uint32_t)(((n - 1) * (int)g.cache.v_row + g.cache.dim) * 2) : 0u);
+      const pk_u32x4 rs = rsrc_words(base + (int64_t)(n > 0 ? page : 0) * page_stride + row * row_stride,
+                                     n > 0 ? (uint32_t)(((n - 1) * (int)row_stride + g.cache.dim) * 2) : 0u);
 #pragma unroll
-      for (int i = 0; i < NI; ++i) dma_lds16<NT>(kr, ks + i * 1024, kvo[i], 0);
-#pragma unroll
-      for (int i = 0; i < NI; ++i) dma_lds16<NT>(vr, vs + i * 1024, vvo[i], 0);
+      for (int i = 0; i < NI; ++i) dma_lds16<NT>(rs, to + i * 1024, offset[i], 0);
     } else {
-      const uint16_t *kp[NI], *vp[NI];
+      const uint16_t *src[NI];
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
         const int row = row_of(i), page = __shfl(pages, (t % BATCH) * 16 + row, 64);
-        const bool is = row < left && page >= 0;
+        const bool is = row < left && page >= 0 && 8 * chunk(i) < g.cache.dim;
         const int at = is ? key + row - (int)(g.cache.page.div(key + row) * g.cache.page.d) : 0;
-        const uint16_t *zero = reinterpret_cast<const uint16_t *>(pd_zeros);
-        kp[i] = is && 8 * k_chunk(i) < g.cache.dim ? kbase + page * g.cache.k_page + at * g.cache.k_row + 8 * k_chunk(i) : zero;
-        vp[i] = is && 8 * v_chunk(i) < g.cache.dim ? vbase + page * g.cache.v_page + at * g.cache.v_row + 8 * v_chunk(i) : zero;
+        src[i] = is ? base + page * page_stride + at * row_stride + 8 * chunk(i) : reinterpret_cast<const uint16_t *>(pd_zeros);
       }
 #pragma unroll
-      for (int i = 0; i < NI; ++i) dma_lds16_at(kp[i], ks + i * 1024);
-#pragma unroll
-      for (int i = 0; i < NI; ++i) dma_lds16_at(vp[i], vs + i * 1024);
+      for (int i = 0; i < NI; ++i) dma_lds16_at(src[i], to + i * 1024);
     }
   }
-  // Which keys of tile t (the last one issued) are on pages that are there, a bit each.
+  // Which keys of tile t (the last one of K issued) are on pages that are there, a bit each.
   __device__ __forceinline__ uint32_t there(int t) const {
-    if constexpr (PAGE16) return __builtin_amdgcn_readlane(pages, t % BATCH) < 0 ? 0u : 0xFFFFu;
-    else return (uint32_t)(__ballot(pages >= 0) >> (16 * (t % BATCH))) & 0xFFFFu;
+    if constexpr (PAGE16) return __builtin_amdgcn_readlane(kpages, t % BATCH) < 0 ? 0u : 0xFFFFu;
+    else return (uint32_t)(__ballot(kpages >= 0) >> (16 * (t % BATCH))) & 0xFFFFu;
   }
 };
 
@@ -146,14 +148,28 @@ __device__ __forceinline__ pk_u16x2 exponents(pk_u16x2 most, uint32_t w) {
 }
 __device__ __forceinline__ bool not_finite(pk_u16x2 most) { return most.x >= 0x7F80 || most.y >= 0x7F80; }
 
-// A value (low half of w) for the passes over a tile with values that are no numbers: 0
-// keeps the finite ones, 1 and 2 hold 2^127 and -2^127 where it is +inf and -inf, both
-// for a NaN.
-__device__ __forceinline__ uint32_t apart_half(uint32_t w, int pass) {
-  const bool finite = (w & 0x7F80u) != 0x7F80u, nan = !finite && (w & 0x7Fu);
-  if (pass == 0) return finite ? w & 0xFFFFu : 0u;
-  if (pass == 1) return nan || (w & 0xFFFFu) == 0x7F80u ? 0x7F00u : 0u;
-  return nan || (w & 0xFFFFu) == 0xFF80u ? 0xFF00u : 0u;
+// A hidden key's value that is no number must not meet its zero weight in a product.  Where
+// some rows see such a key and others don't, the products take zero for it (`finite`), and
+// the rows that see it get it at the end (`add_not_finite`).
+__device__ __forceinline__ uint32_t finite(uint32_t w) {
+  const uint32_t lo = (w & 0x7F80u) == 0x7F80u ? 0u : 0xFFFFu, hi = (w & 0x7F800000u) == 0x7F800000u ? 0u : 0xFFFF0000u;
+  return w & (lo | hi);
+}
+// Adds the values of key `key` at `at` that are infinite or no number to four sums.
+__device__ __forceinline__ void add_not_finite(const uint16_t *at, f32x4 &sum) {
+  const att::u32x2 w = *reinterpret_cast<const att::u32x2 *>(at);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t v = (i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
+    if ((v & 0x7F800000u) == 0x7F800000u) sum[i] += __uint_as_float(v);
+  }
+}
+// The values of key `key` of one head, or null where its page is not there.
+__device__ __forceinline__ const uint16_t *value_row(const AttendArgs &g, int b, int hk, int key) {
+  const int page = page_of(g.batch, g.cache, b, key);
+  if (page < 0) return nullptr;
+  return g.cache.v + hk * g.cache.v_head + page * g.cache.v_page +
+         (key - (int)(g.cache.page.div(key) * g.cache.page.d)) * g.cache.v_row;
 }
 
 }  // namespace paged
