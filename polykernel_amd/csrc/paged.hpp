@@ -81,10 +81,14 @@ __device__ __forceinline__ int sequence_of(const Batch &g, int t) {
   return n < g.sequences && g.q_start[n] <= t ? n : -1;
 }
 
-// The page of position p (0 <= p < capacity), or -1.
+// The page of position p (0 <= p < capacity) as the table has it, and that number where
+// there is such a page, else -1.
+__device__ __forceinline__ int page_number(const Batch &g, const Cache &c, int b, int p) {
+  return g.page_table[b * g.table_stride + c.page.div(p)];
+}
+__device__ __forceinline__ int page_or_none(const Cache &c, int page) { return (unsigned)page < (unsigned)c.pages ? page : -1; }
 __device__ __forceinline__ int page_of(const Batch &g, const Cache &c, int b, int p) {
-  const int page = g.page_table[b * g.table_stride + c.page.div(p)];
-  return (unsigned)page < (unsigned)c.pages ? page : -1;
+  return page_or_none(c, page_number(g, c, b, p));
 }
 
 // ---- argument checks -------------------------------------------------------

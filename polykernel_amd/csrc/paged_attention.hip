@@ -103,7 +103,7 @@ __global__ __launch_bounds__(PD_THREADS) void paged_decode_merge_kernel(DecodeAr
   paged_decode_merge_body<DP, MT>(d);
 }
 template <int DP, bool PAGE16>
-__global__ __launch_bounds__(PC_THREADS, DP == 256 ? 1 : 2) void paged_chunk_kernel(ChunkArgs d) {
+__global__ __launch_bounds__(PC_THREADS, DP == 256 ? 1 : DP == 64 ? 3 : 2) void paged_chunk_kernel(ChunkArgs d) {
   paged_chunk_body<DP, PAGE16>(d);
 }
 template <int DP>
@@ -163,7 +163,8 @@ Choice choose(int q_heads, const pk_paged_cache &c, const pk_paged_batch &b) {
 
 bool tile_operands(const AttendArgs &g) {
   const Cache &c = g.cache;
-  auto rows = [&](int64_t row) { return row >= c.dim && row < (int64_t(1) << 26); };
+  // row offsets within a page, in bytes, and the length of 16 rows are 32-bit numbers
+  auto rows = [&](int64_t row) { return row >= c.dim && row < (int64_t(1) << 26) && row * 2 * c.page.d < (int64_t(1) << 32); };
   return aligned16(g.q.data) && aligned16(g.out.data) && aligned16(c.k) && aligned16(c.v) &&
          strides8(g.q.token, g.q.head) && strides8(g.out.token, g.out.head) && strides8(c.k_page, c.k_head, c.k_row) &&
          strides8(c.v_page, c.v_head, c.v_row) && rows(c.k_row) && rows(c.v_row);

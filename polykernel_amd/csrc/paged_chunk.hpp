@@ -96,7 +96,7 @@ __device__ __forceinline__ void lds_barrier() {
 
 template <int DP>
 struct ChunkShape {
-  static constexpr int TB = PC_STEP * DP * 2, SL = DP == 64 ? 3 : 2;  // tile bytes, slots of a ring
+  static constexpr int TB = PC_STEP * DP * 2, SL = 2;  // bytes of a step, slots of a ring
   static constexpr int OS = DP * 2 + 16;                             // row stride of a wave's rows on their way out
   static constexpr int LDS = 2 * SL * TB;
   static_assert(PC_ROWS * OS <= LDS, "the outputs pass through the rings");
@@ -135,6 +135,16 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
   const int kfirst = klo + s0 * PC_STEP;
   Tiles tiles(g);
   tiles.begin(g, it.b, it.hk, kfirst + wid * PT_KEYS, nst, hi_last);
+  // PAGE16: a lane per tile, four a step: pages of 16 steps, and of the 16 after them
+  auto pages_of = [&](int t) __attribute__((always_inline)) {
+    const int key = kfirst + t * PC_STEP + lane * PT_KEYS;
+    return t < nst && key < hi_last ? page_number(g.batch, g.cache, it.b, key) : -1;
+  };
+  int pages = -1, pages_next = -1, v_page = 0, v_row = 0, v_n = 0;
+  uint64_t pages_there = 0;  // of `pages`
+  if constexpr (PAGE16) {
+    pages_next = pages_of(0);
+  }
   int lo_all, hi_all, t2, t3;
   key_range(g, s, (int)g.group.div(min(wrow, all_rows - 1)), t2, hi_all);
   key_range(g, s, (int)g.group.div(min(wrow + 31, all_rows - 1)), lo_all, t3);
@@ -165,16 +175,36 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
   for (int e = 0; e < VO; ++e)
     vo[e] = (uint32_t)((4 * h + (gi >> 2)) * RB + 16 * ((4 * e + 2 * (grp & 1) + ((gi & 3) >> 1)) ^ att::swz_v<DP>(gi >> 2)) + 8 * (gi & 1));
 
-  // K of step t and V of step t lie in slot t % SL of their rings.  Step t's iteration reads K
-  // of step t + 1 and V of step t, and loads K of step t + SL (K of step t has been read) and
-  // V of step t + SL - 1 (V of step t - 1 has).
+  // K of step t and V of step t lie in slot t % 2 of their rings.  Step t's iteration reads K
+  // of step t + 1 and V of step t, and loads V of step t + 1 (V of step t - 1 has been read)
+  // and K of step t + 2 (K of step t has).
+  // Steps of K from 0 on, and a step's V after its K and before the next one's.
+  const uint32_t ring_at = lds_number(ring) + wid * Tiles::BYTES;
+  uint32_t there_bits[SL];  // PAGE16: tiles of the step in a slot of K that are there, 4 bits
   auto issue_k = [&](int t, int sl) __attribute__((always_inline)) {
-    tiles.issue_k(g, t, ring + sl * TB + wid * Tiles::BYTES);
-    const uint32_t is = tiles.there(t);  // by all lanes
-    if (lane == 0) there_s[sl][wid] = (uint16_t)is;
+    if constexpr (PAGE16) {
+      if (t % 16 == 0) {
+        pages = page_or_none(g.cache, pages_next);
+        pages_there = __ballot(pages >= 0);
+        pages_next = pages_of(t + 16);
+      }
+      const int page = __builtin_amdgcn_readlane(pages, 4 * (t % 16) + wid), key = kfirst + t * PC_STEP + wid * PT_KEYS;
+      v_n = t < nst && page >= 0 ? min(PT_KEYS, hi_last - key) : 0;
+      v_row = key - (int)(g.cache.page.div(key) * g.cache.page.d);
+      v_page = v_n > 0 ? page : 0;
+      there_bits[sl] = (uint32_t)(pages_there >> (4 * (t % 16))) & 15u;
+      Tiles::load_rows(g, v_page, v_row, v_n, tiles.kbase, g.cache.k_page, g.cache.k_row, tiles.kvo, ring_at + sl * TB);
+    } else {
+      tiles.issue_k(g, t, ring_at + sl * TB);
+      const uint32_t is = tiles.there(t);  // by all lanes
+      if (lane == 0) there_s[sl][wid] = (uint16_t)is;
+    }
   };
   auto issue_v = [&](int t, int sl) __attribute__((always_inline)) {
-    tiles.issue_v(g, t, ring + (SL + sl) * TB + wid * Tiles::BYTES);
+    if constexpr (PAGE16)
+      Tiles::load_rows(g, v_page, v_row, v_n, tiles.vbase, g.cache.v_page, g.cache.v_row, tiles.vvo, ring_at + (SL + sl) * TB);
+    else
+      tiles.issue_v(g, t, ring_at + (SL + sl) * TB);
   };
 
   f32x16 acc[DB], sc[2];
@@ -204,19 +234,23 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
     return __builtin_bit_cast(bf16x8, __builtin_shufflevector(hv[0], hv[1], 0, 1, 2, 3, 4, 5, 6, 7));
   };
   // Scores of the step in K slot sl, and beside product i the work of `beside(i)`.  Fragments
-  // are read AHEAD products before they are used, and the order is kept as written.
+  // are read AHEAD products before they are used, and the order of pairs is kept as written.
   constexpr int AHEAD = 4, NA = 2 * DS, NB = 4 * DB;
   auto scores = [&](int sl, f32x16 (&x)[2], auto beside) __attribute__((always_inline)) {
     bf16x8 f[NA];
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) f[i] = k_fragment(sl, i);
+    x[0] = x[1] = f32x16{};
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < NA; ++i) {
-      if (i < 2) x[i] = f32x16{};
-      x[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[i], qf[i >> 1], x[i & 1], 0, 0, 0);
-      if (i + AHEAD < NA) f[i + AHEAD] = k_fragment(sl, i + AHEAD);
-      beside(i);
+    for (int i = 0; i < NA; i += 2) {
+#pragma unroll
+      for (int j = i; j < i + 2; ++j) {
+        x[j & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[j], qf[j >> 1], x[j & 1], 0, 0, 0);
+        beside(j);
+      }
+#pragma unroll
+      for (int j = i + AHEAD; j < min(NA, i + AHEAD + 2); ++j) f[j] = k_fragment(sl, j);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -230,10 +264,19 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
   };
   // hides what this wave's rows do not see of step t, whose scores are in sc (K slot sl)
   auto mask = [&](int t, int sl) __attribute__((always_inline)) {
-    const att::u32x2 w = *reinterpret_cast<const att::u32x2 *>(there_s[sl]);
-    const uint32_t there[2] = {(uint32_t)uniform((int)w[0]), (uint32_t)uniform((int)w[1])};
     const int key = kfirst + t * PC_STEP;
-    whole = (there[0] & there[1]) == 0xFFFFFFFFu;
+    uint32_t there[2];
+    if constexpr (PAGE16) {
+      const uint32_t f = there_bits[sl];
+      whole = f == 15u;
+      there[0] = (f & 1 ? 0xFFFFu : 0u) | (f & 2 ? 0xFFFF0000u : 0u);
+      there[1] = (f & 4 ? 0xFFFFu : 0u) | (f & 8 ? 0xFFFF0000u : 0u);
+    } else {
+      const att::u32x2 w = *reinterpret_cast<const att::u32x2 *>(there_s[sl]);
+      there[0] = (uint32_t)uniform((int)w[0]);
+      there[1] = (uint32_t)uniform((int)w[1]);
+      whole = (there[0] & there[1]) == 0xFFFFFFFFu;
+    }
     if (key < lo_all || key + PC_STEP > hi_all || !whole) {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
@@ -252,15 +295,15 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
   };
 
   auto step = [&](auto slot, int t) __attribute__((always_inline)) {
-    constexpr int sl = decltype(slot)::value, next = (sl + 1) % SL;
-    vm_wait<2 * NI * (SL - 2)>();  // this wave's part of K of step t + 1 and V of step t has landed
-    lds_barrier();                 // and every wave's; nobody reads what the next loads overwrite
+    constexpr int sl = decltype(slot)::value, next = 1 - sl;
+    vm_wait<0>();  // this wave's part of K of step t + 1 and V of step t has landed
+    lds_barrier();  // and every wave's; nobody reads what the next loads overwrite
     uint8_t *const vs = ring + (SL + sl) * TB;
     const int key = kfirst + t * PC_STEP;
     // the same for every wave: whether some row of the item has a hidden key in this step
     const bool mixed = key < t1 || key + PC_STEP > t0 || !whole;
-    issue_k(t + SL, sl);
-    issue_v(t + SL - 1, (sl + SL - 1) % SL);
+    issue_v(t + 1, next);
+    issue_k(t + 2, sl);
 
     // the maximum in the exponent follows once it is 2^8 behind
     if (__any((top - m_run) * c2 > 8.f)) {
@@ -275,19 +318,22 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
     f32x16 nx[2];
     att::u32x4 pw[4];
     float sum = 0.f;
+    // weights of scores 2 n and 2 n + 1: three quarters beside the next scores, the rest beside the
+    // first products with V, which are those of the other weights
+    constexpr int EARLY = 12;
+    auto weights = [&](int n) __attribute__((always_inline)) {
+      const int kb = n >> 3, j = 2 * (n & 7);
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[kb][j], c2, -mc));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[kb][j + 1], c2, -mc));
+      sum += p0 + p1;
+      uint32_t two = pack_bf(p0, p1);
+      asm volatile("" : "+v"(two), "+v"(sum));  // here, not where they are used first
+      pw[n >> 2][n & 3] = two;
+    };
     scores(next, nx, [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-      for (int n = i * 16 / NA; n < (i + 1) * 16 / NA; ++n) {  // two of the 32 scores
-        const int kb = n >> 3, j = 2 * (n & 7);
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[kb][j], c2, -mc));
-        const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[kb][j + 1], c2, -mc));
-        sum += p0 + p1;
-        uint32_t two = pack_bf(p0, p1);
-        asm volatile("" : "+v"(two));  // here, not where it is used first
-        pw[n >> 2][n & 3] = two;
-      }
+      for (int n = i * EARLY / NA; n < (i + 1) * EARLY / NA; ++n) weights(n);
     });
-    l_run += sum;
 
     if (mixed) {
       pk_u16x2 most = {0, 0};
@@ -319,13 +365,21 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
       for (int i = 0; i < AHEAD; ++i) f[i] = v_fragment(sl, i);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        acc[i % DB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[i], __builtin_bit_cast(bf16x8, pw[i / DB]), acc[i % DB], 0, 0, 0);
-        if (i + AHEAD < NB) f[i + AHEAD] = v_fragment(sl, i + AHEAD);
+      for (int i = 0; i < NB; i += 2) {
 #pragma unroll
-        for (int n = i * 32 / NB; n < (i + 1) * 32 / NB; ++n) top = fmaxf(top, nx[n >> 4][n & 15]);
+        for (int j = i; j < i + 2; ++j) {
+          acc[j % DB] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f[j], __builtin_bit_cast(bf16x8, pw[j / DB]), acc[j % DB], 0, 0, 0);
+          constexpr int ON = 3 * DB;  // products with the early weights
+#pragma unroll
+          for (int n = EARLY + j * (16 - EARLY) / ON; n < min(16, EARLY + (j + 1) * (16 - EARLY) / ON); ++n) weights(n);
+#pragma unroll
+          for (int n = j * 32 / NB; n < (j + 1) * 32 / NB; ++n) top = fmaxf(top, nx[n >> 4][n & 15]);
+        }
+#pragma unroll
+        for (int j = i + AHEAD; j < min(NB, i + AHEAD + 2); ++j) f[j] = v_fragment(sl, j);
         __builtin_amdgcn_sched_barrier(0);
       }
+      l_run += sum;
       top = xor32_max(top);
     }
     sc[0] = nx[0];
@@ -334,23 +388,20 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
   };
 
   issue_k(0, 0);
-#pragma unroll
-  for (int t = 0; t < SL - 1; ++t) {
-    issue_k(t + 1, t + 1);
-    issue_v(t, t);
-  }
-  vm_wait<2 * NI * (SL - 1)>();
+  issue_v(0, 0);
+  issue_k(1, 1);
+  vm_wait<2 * NI>();
   lds_barrier();
   scores(0, sc, [](int) {});
   top = maximum(sc);
   mask(0, 0);
+  int t = 0;
 #pragma unroll 1
-  for (int t = 0; t < nst; t += SL) {
+  for (; t + 1 < nst; t += 2) {
     step(std::integral_constant<int, 0>{}, t);
-    if (t + 1 < nst) step(std::integral_constant<int, 1>{}, t + 1);
-    if constexpr (SL == 3)
-      if (t + 2 < nst) step(std::integral_constant<int, 2>{}, t + 2);
+    step(std::integral_constant<int, 1>{}, t + 1);
   }
+  if (t < nst) step(std::integral_constant<int, 0>{}, t);
   vm_wait<0>();
   l_run = xor32_sum(l_run);
   for (int k = kfirst + odd_first * PC_STEP; k < min(hi_last, kfirst + (odd_last + 1) * PC_STEP); ++k) {

@@ -153,6 +153,7 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
   const int col = lane & 15, grp = lane >> 4;
   const int D = g.cache.dim;
   uint8_t *const mine = ring + wid * S::WAVE;  // K slots, then V slots
+  const uint32_t mine_at = lds_number(ring) + wid * S::WAVE;
 
   Place at;
   if (!find_place<ROWS>(d, blockIdx.x, at)) return;
@@ -213,8 +214,8 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
     const float c2 = fabsf(g.c2);
 
     auto issue = [&](int t) __attribute__((always_inline)) {
-      tiles.issue_k(g, t, mine + (t % SL) * TB);
-      tiles.issue_v(g, t, mine + (SL + t % SL) * TB);
+      tiles.issue_k(g, t, mine_at + (t % SL) * TB);
+      tiles.issue_v(g, t, mine_at + (SL + t % SL) * TB);
     };
     float m_run[MT], l_run[MT];
     f32x4 acc[MT][DB];

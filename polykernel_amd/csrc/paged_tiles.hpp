@@ -50,13 +50,25 @@ __device__ __forceinline__ int wave_scan(int v) {
 // 16 zero bytes that rows which are not there are read from.
 __device__ const uint32_t pd_zeros[4] __attribute__((aligned(16))) = {0, 0, 0, 0};
 
+// An LDS address as the number that m0 takes.
+__device__ __forceinline__ uint32_t lds_number(const void *p) {
+  return (uint32_t)reinterpret_cast<uintptr_t>((lds_void *)p);
+}
+
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
+// dma_lds16 to a numbered address; resource and address in scalar registers.
+template <bool NT>
+__device__ __forceinline__ void dma_lds16_to(pk_u32x4 rs, uint32_t lds, uint32_t voff) {
+  if constexpr (NT)
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds" : : "s"(lds), "v"(voff), "s"(rs) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(lds), "v"(voff), "s"(rs) : "memory", "m0");
+}
 // global_load_lds_dwordx4: lane i copies 16 bytes from its own address to lds + 16 i
 // (ordered by vm_wait, as dma_lds16).
-__device__ __forceinline__ void dma_lds16_at(const void *src, const void *lds) {
-  const int m0 = __builtin_amdgcn_readfirstlane((int)(uint32_t)reinterpret_cast<uintptr_t>((lds_void *)lds));
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(m0), "v"(src) : "memory", "m0");
+__device__ __forceinline__ void dma_lds16_at(const void *src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(src) : "memory", "m0");
 }
 #pragma clang diagnostic pop
 
@@ -100,27 +112,35 @@ struct TileLoader {
     vbase = g.cache.v + hk * g.cache.v_head;
     kpages = vpages = look_up(g, 0);
   }
-  // Tiles of K, and of V, in order from 0; tiles from `count` on load nothing (as many
-  // instructions, of no length).
-  __device__ __forceinline__ void issue_k(const AttendArgs &g, int t, uint8_t *to) {
+  // Tiles of K, and of V, in order from 0 to the LDS address `to`; tiles from `count` on load
+  // nothing (as many instructions, of no length).
+  __device__ __forceinline__ void issue_k(const AttendArgs &g, int t, uint32_t to) {
     if (t % BATCH == 0 && t > 0 && t < count) kpages = look_up(g, t);
     load(g, t, kpages, kbase, g.cache.k_page, g.cache.k_row, kvo, [](int i) { return k_chunk(i); }, to);
   }
-  __device__ __forceinline__ void issue_v(const AttendArgs &g, int t, uint8_t *to) {
+  __device__ __forceinline__ void issue_v(const AttendArgs &g, int t, uint32_t to) {
     if (t % BATCH == 0 && t > 0 && t < count) vpages = look_up(g, t);
     load(g, t, vpages, vbase, g.cache.v_page, g.cache.v_row, vvo, [](int i) { return v_chunk(i); }, to);
   }
+  // `n` rows from row `row` of a page (none: a resource of no length).
+  __device__ __forceinline__ static void load_rows(const AttendArgs &g, int page, int row, int n, const uint16_t *base,
+                                                   int64_t page_stride, int64_t row_stride, const uint32_t (&offset)[NI],
+                                                   uint32_t to) {
+    const uint64_t p = reinterpret_cast<uint64_t>(base) + 2 * (uint64_t)(uint32_t)page * (uint64_t)page_stride +
+                       (uint32_t)row * (uint32_t)(2 * row_stride);
+    const pk_u32x4 rs = {(uint32_t)uniform((int)(uint32_t)p), (uint32_t)uniform((int)((uint32_t)(p >> 32) & 0xFFFFu)),
+                         (uint32_t)uniform(n > 0 ? ((n - 1) * (int)row_stride + g.cache.dim) * 2 : 0), 0x00020000u};
+#pragma unroll
+    for (int i = 0; i < NI; ++i) dma_lds16_to<NT>(rs, (uint32_t)uniform((int)to + i * 1024), offset[i]);
+  }
   template <typename Chunk>
   __device__ __forceinline__ void load(const AttendArgs &g, int t, int pages, const uint16_t *base, int64_t page_stride,
-                                       int64_t row_stride, const uint32_t (&offset)[NI], Chunk chunk, uint8_t *to) {
+                                       int64_t row_stride, const uint32_t (&offset)[NI], Chunk chunk, uint32_t to) {
     const int key = key0 + t * PT_STEP, left = t < count ? hi - key : 0;
     if constexpr (PAGE16) {
       const int page = __builtin_amdgcn_readlane(pages, t % BATCH), n = page < 0 ? 0 : min(PT_KEYS, left);
       const int row = n > 0 ? key - (int)(g.cache.page.div(key) * g.cache.page.d) : 0;
-      const pk_u32x4 rs = rsrc_words(base + (int64_t)(n > 0 ? page : 0) * page_stride + row * row_stride,
-                                     n > 0 ? (uint32_t)(((n - 1) * (int)row_stride + g.cache.dim) * 2) : 0u);
-#pragma unroll
-      for (int i = 0; i < NI; ++i) dma_lds16<NT>(rs, to + i * 1024, offset[i], 0);
+      load_rows(g, n > 0 ? page : 0, row, n, base, page_stride, row_stride, offset, to);
     } else {
       const uint16_t *src[NI];
 #pragma unroll
@@ -131,7 +151,7 @@ struct TileLoader {
         src[i] = is ? base + page * page_stride + at * row_stride + 8 * chunk(i) : reinterpret_cast<const uint16_t *>(pd_zeros);
       }
 #pragma unroll
-      for (int i = 0; i < NI; ++i) dma_lds16_at(src[i], to + i * 1024);
+      for (int i = 0; i < NI; ++i) dma_lds16_at(src[i], (uint32_t)uniform((int)to + i * 1024));
     }
   }
   // Which keys of tile t (the last one of K issued) are on pages that are there, a bit each.
