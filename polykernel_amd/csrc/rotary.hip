@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "attention_kernels.hpp"
 #include "paged.hpp"
 
 namespace pk {
@@ -42,7 +43,7 @@ int check_batch(const char *who, const pk_paged_batch *b, const pk_paged_cache *
 
 namespace {
 
-constexpr int RO_THREADS = 256, RO_MAX_HALF = 512;
+constexpr int RO_THREADS = 256;
 
 struct Rotation {
   const double *turns;
@@ -50,90 +51,228 @@ struct Rotation {
   float sine, magnitude;  // sine: -1 to turn back
 };
 
-// cos and sin (times the magnitude) of every pair at position p, by the workgroup.
-__device__ __forceinline__ void angles(const Rotation &r, int p, float2 *cs) {
-  for (int i = threadIdx.x; i < r.half; i += RO_THREADS) {
-    const double rev = (double)p * r.turns[i];
-    float s, c;
-    sincospif(2.f * (float)(rev - rint(rev)), &s, &c);
-    cs[i] = make_float2(c * r.magnitude, s * r.sine * r.magnitude);
-  }
+// Work on a head, in units of V dims (16 bytes, or one where strides, alignment or the
+// number of pairs allow no more): the pairs of a unit, or of two units half a rotation
+// apart; then a unit behind the rotated dims.
+template <int V>
+__host__ __device__ __forceinline__ int pieces(int half, int interleaved, int D) {
+  const int rotated = V == 1 ? half : interleaved ? 2 * half / V : half / V;
+  return rotated + (D - 2 * half) / V;
 }
-
-// Pieces of a head: a pair, or one dim behind the rotated ones.
-__host__ __device__ __forceinline__ int pieces(int half, int D) { return D - half; }
-__device__ __forceinline__ void rotate_piece(const Rotation &r, const float2 *cs, const uint16_t *src, uint16_t *dst, int j) {
-  if (j < r.half) {
-    const int d0 = r.interleaved ? 2 * j : j, d1 = r.interleaved ? d0 + 1 : j + r.half;
-    const float a = bf2f(src[d0]), b = bf2f(src[d1]);
-    const float c = cs[j].x, s = cs[j].y;
-    dst[d0] = (uint16_t)f2bf(fmaf(a, c, -(b * s)));
-    dst[d1] = (uint16_t)f2bf(fmaf(b, c, a * s));
-  } else {
-    dst[j + r.half] = src[j + r.half];
-  }
-}
-
-struct RotaryArgs {
-  Heads x, out;
-  const int32_t *positions;
-  int64_t position_stride;
-  int S, heads;
-  FastDiv per_head;
-  Rotation rot;
+template <int V>
+struct Piece {
+  att::u32x4 a, b;  // V 8: the units; V 1: a dim in the low half of each first word
 };
-
-// One token per workgroup.
-__global__ __launch_bounds__(RO_THREADS) void rotary_kernel(RotaryArgs g) {
-  __shared__ float2 cs[RO_MAX_HALF];
-  const int b = blockIdx.x / g.S, s = blockIdx.x % g.S;
-  angles(g.rot, g.positions[b * g.position_stride + s], cs);
-  __syncthreads();
-  const uint16_t *src = g.x.data + b * g.x.batch + s * g.x.token;
-  uint16_t *dst = g.out.data + b * g.out.batch + s * g.out.token;
-  for (int u = threadIdx.x; u < g.heads * (int)g.per_head.d; u += RO_THREADS) {
-    const int h = (int)g.per_head.div(u), j = u - h * (int)g.per_head.d;
-    rotate_piece(g.rot, cs, src + h * g.x.head, dst + h * g.out.head, j);
+// Offsets of piece j's two units in its head (the second is the first where there is one).
+template <int V>
+__device__ __forceinline__ void place(const Rotation &r, int j, int &d0, int &d1, bool &rotated) {
+  if constexpr (V == 1) {
+    rotated = j < r.half;
+    d0 = !rotated ? j + r.half : r.interleaved ? 2 * j : j;
+    d1 = !rotated ? d0 : r.interleaved ? d0 + 1 : j + r.half;
+  } else {
+    const int n = r.interleaved ? 2 * r.half / V : r.half / V;
+    rotated = j < n;
+    d0 = V * (rotated || r.interleaved ? j : j + n);
+    d1 = rotated && !r.interleaved ? d0 + r.half : d0;
+  }
+}
+template <int V>
+__device__ __forceinline__ Piece<V> read_piece(const Rotation &r, const uint16_t *src, int j) {
+  int d0, d1;
+  bool rotated;
+  place<V>(r, j, d0, d1, rotated);
+  Piece<V> p;
+  if constexpr (V == 8) {
+    p.a = __builtin_nontemporal_load(reinterpret_cast<const att::u32x4 *>(src + d0));
+    if (d1 != d0) p.b = __builtin_nontemporal_load(reinterpret_cast<const att::u32x4 *>(src + d1));
+  } else {
+    p.a[0] = src[d0];
+    if (d1 != d0) p.b[0] = src[d1];
+  }
+  return p;
+}
+__device__ __forceinline__ void turn(float2 cs, float a, float b, float &x, float &y) {
+  x = fmaf(a, cs.x, -(b * cs.y));
+  y = fmaf(b, cs.x, a * cs.y);
+}
+// cs: the token's cosines and sines, times the magnitude.
+template <int V>
+__device__ __forceinline__ void write_piece(const Rotation &r, const float2 *cs, Piece<V> p, uint16_t *dst, int j) {
+  int d0, d1;
+  bool rotated;
+  place<V>(r, j, d0, d1, rotated);
+  if constexpr (V == 1) {
+    if (!rotated) {
+      dst[d0] = (uint16_t)p.a[0];
+      return;
+    }
+    float x, y;
+    turn(cs[j], bf2f(p.a[0]), bf2f(p.b[0]), x, y);
+    dst[d0] = (uint16_t)f2bf(x);
+    dst[d1] = (uint16_t)f2bf(y);
+  } else {
+    if (rotated && r.interleaved) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float x, y;
+        turn(cs[4 * j + e], lo_bf(p.a[e]), hi_bf(p.a[e]), x, y);
+        p.a[e] = pack_bf(x, y);
+      }
+    } else if (rotated) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float x0, y0, x1, y1;
+        turn(cs[8 * j + 2 * e], lo_bf(p.a[e]), lo_bf(p.b[e]), x0, y0);
+        turn(cs[8 * j + 2 * e + 1], hi_bf(p.a[e]), hi_bf(p.b[e]), x1, y1);
+        p.a[e] = pack_bf(x0, x1);
+        p.b[e] = pack_bf(y0, y1);
+      }
+      *reinterpret_cast<att::u32x4 *>(dst + d1) = p.b;
+    }
+    *reinterpret_cast<att::u32x4 *>(dst + d0) = p.a;
   }
 }
 
-struct AppendArgs {
-  Heads k, v, q, q_out;
+struct RotateArgs {
+  Heads q, q_out;          // what is rotated from tensor to tensor
+  Heads k, v;              // append: new keys and values
   Cache cache;
   Batch batch;
-  int q_heads;  // 0: no queries
-  FastDiv per_head, per_value;
+  const int32_t *positions;  // rotary: of token (b, s) at b * position_stride + s
+  int64_t position_stride;
+  int tokens;
+  int per_group;             // tokens of a workgroup
+  FastDiv of_token, of_head, of_value;  // pieces of a token, of a rotated head, of a value head
+  FastDiv of_entry;                     // rotary: tokens of a batch entry
+  int q_pieces, k_pieces;
   Rotation rot;
 };
 
-// One new token per workgroup: its query heads, key heads and value heads.
-__global__ __launch_bounds__(RO_THREADS) void paged_append_kernel(AppendArgs g) {
-  __shared__ float2 cs[RO_MAX_HALF];
-  const int t = blockIdx.x;
-  const int b = sequence_of(g.batch, t);
-  if (b < 0) return;
-  const Seq sq = sequence(g.batch, b);
-  const int p = sq.kv - sq.n + t - sq.q0;
-  angles(g.rot, p, cs);
-  const int page = p >= 0 && p < g.batch.capacity ? page_of(g.batch, g.cache, b, p) : -1;
-  const int row = page >= 0 ? p - (int)(g.cache.page.div(p) * g.cache.page.d) : 0;
-  __syncthreads();
-  const int nq = g.q_heads * (int)g.per_head.d;
-  const int nk = page >= 0 ? g.cache.heads * (int)g.per_head.d : 0, nv = page >= 0 ? g.cache.heads * (int)g.per_value.d : 0;
-  uint16_t *kc = g.cache.k + page * g.cache.k_page + row * g.cache.k_row;
-  uint16_t *vc = g.cache.v + page * g.cache.v_page + row * g.cache.v_row;
-  for (int u = threadIdx.x; u < nq + nk + nv; u += RO_THREADS) {
-    if (u < nq) {
-      const int h = (int)g.per_head.div(u), j = u - h * (int)g.per_head.d;
-      rotate_piece(g.rot, cs, g.q.data + t * g.q.token + h * g.q.head, g.q_out.data + t * g.q_out.token + h * g.q_out.head, j);
-    } else if (u < nq + nk) {
-      const int h = (int)g.per_head.div(u - nq), j = u - nq - h * (int)g.per_head.d;
-      rotate_piece(g.rot, cs, g.k.data + t * g.k.token + h * g.k.head, kc + h * g.cache.k_head, j);
+// A workgroup takes `per_group` tokens: their positions and places (a wave per token),
+// the angles of all pairs, then the pieces of all heads.  What bounds it: the memory, 2 x
+// 16 bytes in and out per piece; the first piece of a thread is read before the places
+// are known, which hides most of that chain of reads in a call of few tokens.
+constexpr int RO_TOKENS = 4;
+template <int V, bool APPEND>
+__global__ __launch_bounds__(RO_THREADS) void rotate_kernel(RotateArgs g) {
+  extern __shared__ float2 cs[];  // [per_group][half]
+  __shared__ int pos_s[RO_TOKENS], page_s[RO_TOKENS], row_s[RO_TOKENS];
+  const int t0 = blockIdx.x * g.per_group, n = min(g.per_group, g.tokens - t0);
+  const int tid = threadIdx.x, units = n * (int)g.of_token.d;
+  // where piece u comes from, and its number in its head
+  struct From {
+    const uint16_t *head;
+    int token, piece, h, kind;  // kind 0: query, 1: key, 2: value
+  };
+  auto from = [&](int u) __attribute__((always_inline)) {
+    From f;
+    f.token = (int)g.of_token.div(u);
+    int w = u - f.token * (int)g.of_token.d;
+    const int t = t0 + f.token;
+    f.kind = !APPEND || w < g.q_pieces ? 0 : w < g.q_pieces + g.k_pieces ? 1 : 2;
+    w -= f.kind == 0 ? 0 : f.kind == 1 ? g.q_pieces : g.q_pieces + g.k_pieces;
+    const FastDiv &per = f.kind == 2 ? g.of_value : g.of_head;
+    f.h = (int)per.div(w);
+    f.piece = w - f.h * (int)per.d;
+    const Heads &x = f.kind == 0 ? g.q : f.kind == 1 ? g.k : g.v;
+    if constexpr (APPEND) {
+      f.head = x.data + t * x.token + f.h * x.head;
     } else {
-      const int h = (int)g.per_value.div(u - nq - nk), j = u - nq - nk - h * (int)g.per_value.d;
-      vc[h * g.cache.v_head + j] = g.v.data[t * g.v.token + h * g.v.head + j];
+      const int b = (int)g.of_entry.div(t);
+      f.head = x.data + b * x.batch + (t - b * (int)g.of_entry.d) * x.token + f.h * x.head;
+    }
+    return f;
+  };
+  const Rotation none{nullptr, 0, 0, 0.f, 0.f};
+  auto read = [&](const From &f) __attribute__((always_inline)) {
+    return read_piece<V>(f.kind == 2 ? none : g.rot, f.head, f.piece);
+  };
+  From f{};
+  Piece<V> p;
+  if (tid < units) {
+    f = from(tid);
+    p = read(f);
+  }
+
+  const int wid = tid >> 6;
+  if (wid < n) {
+    const int t = t0 + wid;
+    int pos = 0, page = -1, row = 0;
+    if constexpr (APPEND) {
+      const int b = sequence_of(g.batch, t);
+      if (b >= 0) {
+        const Seq s = sequence(g.batch, b);
+        pos = s.kv - s.n + t - s.q0;
+        page = pos >= 0 && pos < g.batch.capacity ? page_of(g.batch, g.cache, b, pos) : -1;
+        row = page >= 0 ? pos - (int)(g.cache.page.div(pos) * g.cache.page.d) : 0;
+      } else {
+        page = -2;  // behind the last sequence: the query is left alone too
+      }
+    } else {
+      const int b = (int)g.of_entry.div(t);
+      pos = g.positions[b * g.position_stride + (t - b * (int)g.of_entry.d)];
+    }
+    if ((tid & 63) == 0) {
+      pos_s[wid] = pos;
+      page_s[wid] = page;
+      row_s[wid] = row;
     }
   }
+  __syncthreads();
+  for (int i = tid; i < n * g.rot.half; i += RO_THREADS) {
+    const int k = i / g.rot.half;
+    const double rev = (double)pos_s[k] * g.rot.turns[i - k * g.rot.half];
+    float s, c;
+    sincospif(2.f * (float)(rev - rint(rev)), &s, &c);
+    cs[i] = make_float2(c * g.rot.magnitude, s * g.rot.sine * g.rot.magnitude);
+  }
+  __syncthreads();
+
+  for (int u = tid; u < units; u += RO_THREADS) {
+    const float2 *token_cs = cs + f.token * g.rot.half;
+    const int t = t0 + f.token, page = page_s[f.token], row = row_s[f.token];
+    if (f.kind == 0) {
+      uint16_t *dst;
+      if constexpr (APPEND) {
+        dst = g.q_out.data + t * g.q_out.token + f.h * g.q_out.head;
+      } else {
+        const int b = (int)g.of_entry.div(t);
+        dst = g.q_out.data + b * g.q_out.batch + (t - b * (int)g.of_entry.d) * g.q_out.token + f.h * g.q_out.head;
+      }
+      if (!APPEND || page != -2) write_piece<V>(g.rot, token_cs, p, dst, f.piece);
+    } else if (page >= 0) {
+      if (f.kind == 1)
+        write_piece<V>(g.rot, token_cs, p, g.cache.k + page * g.cache.k_page + f.h * g.cache.k_head + row * g.cache.k_row, f.piece);
+      else
+        write_piece<V>(none, token_cs, p, g.cache.v + page * g.cache.v_page + f.h * g.cache.v_head + row * g.cache.v_row, f.piece);
+    }
+    if (u + RO_THREADS < units) {
+      f = from(u + RO_THREADS);
+      p = read(f);
+    }
+  }
+}
+
+// Fills in the pieces and launches; `wide`: strides and addresses allow 16-byte pieces.
+template <bool APPEND>
+int run_rotate(RotateArgs g, int q_heads, int kv_heads, int D, bool wide, const char *who, hipStream_t st) {
+  wide = wide && D % 8 == 0 && g.rot.half % (g.rot.interleaved ? 4 : 8) == 0;
+  const int per_head = wide ? pieces<8>(g.rot.half, g.rot.interleaved, D) : pieces<1>(g.rot.half, g.rot.interleaved, D);
+  const int per_value = wide ? D / 8 : D;
+  g.q_pieces = q_heads * per_head;
+  g.k_pieces = kv_heads * per_head;
+  const int total = g.q_pieces + g.k_pieces + kv_heads * per_value;
+  g.of_head = FastDiv((uint32_t)per_head);
+  g.of_value = FastDiv((uint32_t)per_value);
+  g.of_token = FastDiv((uint32_t)total);
+  g.per_group = g.tokens >= 4096 && total <= INT32_MAX / (2 * RO_TOKENS) ? RO_TOKENS : 1;
+  const unsigned blocks = (unsigned)((g.tokens + (int64_t)g.per_group - 1) / g.per_group);
+  const size_t lds = (size_t)g.per_group * g.rot.half * sizeof(float2);
+  if (wide) rotate_kernel<8, APPEND><<<blocks, RO_THREADS, lds, st>>>(g);
+  else rotate_kernel<1, APPEND><<<blocks, RO_THREADS, lds, st>>>(g);
+  PK_LAUNCH_CHECK(who);
+  return PK_OK;
 }
 
 int check_rotary(const char *who, const pk_rotary *r, int D, Rotation *out) {
@@ -195,28 +334,27 @@ int launch_rotary(const uint16_t *x, const int64_t *xs, uint16_t *out, const int
     set_error("launch_rotary: head dim %d > 1024 is not supported", D);
     return PK_ERR_UNSUPPORTED;
   }
-  RotaryArgs g{};
+  RotateArgs g{};
   if (int rc = check_rotary("launch_rotary", rotary, D, &g.rot)) return rc;
-  PK_CHECK_ARG(tokens <= INT32_MAX && (int64_t)H * D <= INT32_MAX, "launch_rotary: B * S = %lld or H * D = %lld exceeds %d",
-               (long long)tokens, (long long)H * D, INT32_MAX);
+  PK_CHECK_ARG(tokens <= INT32_MAX && (int64_t)H * D <= INT32_MAX - 1023,
+               "launch_rotary: B * S = %lld exceeds %d, or H * D = %lld is within 1023 of it", (long long)tokens, INT32_MAX,
+               (long long)H * D);
   if (tokens == 0 || H == 0) return PK_OK;
   PK_CHECK_ARG(x && out && positions, "launch_rotary: null tensor pointer");
-  g.x = Heads{const_cast<uint16_t *>(x), xs[0], xs[1], xs[2]};
-  g.out = Heads{out, os[0], os[1], os[2]};
+  g.q = Heads{const_cast<uint16_t *>(x), xs[0], xs[1], xs[2]};
+  g.q_out = Heads{out, os[0], os[1], os[2]};
   g.positions = positions;
   g.position_stride = position_stride;
-  g.S = S;
-  g.heads = H;
-  g.per_head = FastDiv((uint32_t)pieces(g.rot.half, D));
-  rotary_kernel<<<(unsigned)tokens, RO_THREADS, 0, (hipStream_t)stream>>>(g);
-  PK_LAUNCH_CHECK("rotary_kernel");
-  return PK_OK;
+  g.of_entry = FastDiv((uint32_t)S);
+  g.tokens = (int)tokens;
+  const bool wide = aligned16(x) && aligned16(out) && strides8(xs[0], xs[1], xs[2]) && strides8(os[0], os[1], os[2]);
+  return run_rotate<false>(g, H, 0, D, wide, "rotate_kernel", (hipStream_t)stream);
 }
 
 int launch_paged_kv_append(const pk_tokens *k, const pk_tokens *v, const pk_tokens *q, const pk_tokens *q_out, int q_heads,
                            const pk_paged_cache *cache, const pk_paged_batch *batch, const pk_rotary *rotary, void *stream) {
   const char *who = "launch_paged_kv_append";
-  AppendArgs g{};
+  RotateArgs g{};
   if (int rc = check_cache(who, cache, &g.cache)) return rc;
   if (int rc = check_batch(who, batch, cache, &g.batch)) return rc;
   PK_CHECK_ARG(k && v, "%s: null k or v", who);
@@ -225,9 +363,9 @@ int launch_paged_kv_append(const pk_tokens *k, const pk_tokens *v, const pk_toke
   PK_CHECK_ARG(!rotary || !rotary->inverse, "%s: the inverse rotation is not an append", who);
   if (rotary)
     if (int rc = check_rotary(who, rotary, cache->dim, &g.rot)) return rc;
-  g.q_heads = q ? q_heads : 0;
-  PK_CHECK_ARG(((int64_t)g.q_heads + 2 * (int64_t)cache->heads) * cache->dim <= INT32_MAX, "%s: %d + 2 x %d heads of %d", who,
-               g.q_heads, cache->heads, cache->dim);
+  if (!q) q_heads = 0;
+  PK_CHECK_ARG(((int64_t)q_heads + 2 * (int64_t)cache->heads) * cache->dim <= INT32_MAX - 1023, "%s: %d + 2 x %d heads of %d",
+               who, q_heads, cache->heads, cache->dim);
   if (batch->tokens == 0 || batch->sequences == 0) return PK_OK;
   PK_CHECK_ARG(k->data && v->data && (!q || (q->data && q_out->data)), "%s: null tensor pointer", who);
   g.k = Heads{k->data, 0, k->token, k->head};
@@ -236,11 +374,12 @@ int launch_paged_kv_append(const pk_tokens *k, const pk_tokens *v, const pk_toke
     g.q = Heads{q->data, 0, q->token, q->head};
     g.q_out = Heads{q_out->data, 0, q_out->token, q_out->head};
   }
-  g.per_head = FastDiv((uint32_t)pieces(g.rot.half, cache->dim));
-  g.per_value = FastDiv((uint32_t)cache->dim);
-  paged_append_kernel<<<(unsigned)batch->tokens, RO_THREADS, 0, (hipStream_t)stream>>>(g);
-  PK_LAUNCH_CHECK("paged_append_kernel");
-  return PK_OK;
+  g.tokens = batch->tokens;
+  bool wide = aligned16(k->data) && aligned16(v->data) && aligned16(cache->k) && aligned16(cache->v) &&
+              strides8(k->token, k->head) && strides8(v->token, v->head) &&
+              strides8(cache->k_page, cache->k_head, cache->k_row) && strides8(cache->v_page, cache->v_head, cache->v_row);
+  if (q) wide = wide && aligned16(q->data) && aligned16(q_out->data) && strides8(q->token, q->head) && strides8(q_out->token, q_out->head);
+  return run_rotate<true>(g, q_heads, cache->heads, cache->dim, wide, "rotate_kernel", (hipStream_t)stream);
 }
 
 }  // extern "C"

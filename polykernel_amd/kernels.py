@@ -268,22 +268,25 @@ def _elsewhere(t: torch.Tensor, name: str, dev: int) -> Exception:
 
 def _heads(t: torch.Tensor, dims: int, name: str, dev: int) -> Tuple[int, ...]:
     """The strides of a bf16 tensor of heads on device `dev`: any, with head dims contiguous."""
+    if isinstance(t, torch.Tensor) and t.dtype is bf16 and t.get_device() == dev:
+        strides = t.stride()
+        if len(strides) == dims and (strides[-1] == 1 or t.shape[-1] <= 1):
+            return strides
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch.Tensor")
     if t.dtype != bf16:
         raise TypeError(f"{name}: expected {bf16}, got {t.dtype}")
-    strides = t.stride()
-    if len(strides) != dims:
+    if t.dim() != dims:
         raise ValueError(f"{name}: expected {dims} dimensions, got shape {tuple(t.shape)}")
     if t.get_device() != dev:
         raise _elsewhere(t, name, dev)
-    if strides[-1] != 1 and t.shape[-1] > 1:
-        raise ValueError(f"{name}: the head dim must be contiguous (strides {strides})")
-    return strides
+    raise ValueError(f"{name}: the head dim must be contiguous (strides {t.stride()})")
 
 
 def _table(t: torch.Tensor, shape, dtype: torch.dtype, name: str, dev: int) -> int:
     """A contiguous table of the given shape on device `dev`."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == dev and t.is_contiguous():
+        return t.data_ptr()
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name}: expected a torch.Tensor")
     if t.dtype != dtype:
@@ -292,15 +295,16 @@ def _table(t: torch.Tensor, shape, dtype: torch.dtype, name: str, dev: int) -> i
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.get_device() != dev:
         raise _elsewhere(t, name, dev)
-    if not t.is_contiguous():
-        raise ValueError(f"{name}: tensor must be contiguous")
-    return t.data_ptr()
+    raise ValueError(f"{name}: tensor must be contiguous")
+
+
+# a result's memory: 1.6 us where torch.empty with a shape, type and device takes 3.7
+def _result(like: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(like, memory_format=torch.contiguous_format)
 
 
 def _rotation(turns: torch.Tensor, interleaved: bool, inverse: bool, magnitude: float, dev: int) -> _lib.Rotary:
-    if isinstance(turns, torch.Tensor) and turns.dim() != 1:
-        raise ValueError(f"turns: expected one dimension, got shape {tuple(turns.shape)}")
-    n = turns.shape[0] if isinstance(turns, torch.Tensor) else 0
+    n = turns.numel() if isinstance(turns, torch.Tensor) else 0
     return _lib.Rotary(_table(turns, (n,), torch.float64, "turns", dev), 2 * n, interleaved, inverse, magnitude)
 
 
@@ -318,7 +322,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, turns: torch.Tensor, *, int
     dev, dims = _device(), x.dim()
     xs = _heads(x, dims, "x", dev)
     if out is None:
-        out = torch.empty(x.shape, dtype=bf16, device=x.device)
+        out = _result(x)
         os_ = out.stride()
     else:
         os_ = _heads(out, dims, "out", dev)
@@ -344,11 +348,12 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, turns: torch.Tensor, *, int
 _strides3 = _lib.I64 * 3
 
 
-def _tokens(t: torch.Tensor, name: str, heads: Optional[int], dim: int, tokens: int, dev: int) -> _lib.Tokens:
+def _tokens(t: torch.Tensor, name: str, heads: int, dim: int, tokens: int, dev: int) -> _lib.Tokens:
+    """A [tokens, heads, dim] tensor (heads 0: any number)."""
     strides = _heads(t, 3, name, dev)
-    shape = t.shape
-    if shape[0] != tokens or shape[2] != dim or (heads is not None and shape[1] != heads):
-        raise ValueError(f"{name}: expected [{tokens}, {'heads' if heads is None else heads}, {dim}], got {tuple(shape)}")
+    n, h, d = t.shape
+    if n != tokens or d != dim or (heads and h != heads):
+        raise ValueError(f"{name}: expected [{tokens}, {heads or 'heads'}, {dim}], got {tuple(t.shape)}")
     return _lib.Tokens(t.data_ptr(), strides[0], strides[1])
 
 
@@ -357,14 +362,14 @@ def _paged(k_cache, v_cache, page_table, q_start, kv_len, tokens: int, max_q: in
     shape = k_cache.shape
     if shape != v_cache.shape:
         raise ValueError(f"k_cache and v_cache must have the same shape, got {tuple(shape)}, {tuple(v_cache.shape)}")
-    cache = _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], shape[0],
-                            shape[2], shape[1], shape[3])
+    pages, heads, rows, dim = shape
+    cache = _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), *ks[:3], *vs[:3], pages, rows, heads, dim)
     if not isinstance(kv_len, torch.Tensor) or kv_len.dim() != 1:
         raise ValueError("kv_len: expected an int32 tensor [sequences]")
     B = kv_len.shape[0]
     if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2 or page_table.shape[0] != B:
         raise ValueError(f"page_table: expected an int32 tensor [{B}, pages of a sequence]")
-    if page_table.dtype != torch.int32:
+    if page_table.dtype is not torch.int32:
         raise TypeError(f"page_table: expected {torch.int32}, got {page_table.dtype}")
     if page_table.get_device() != dev:
         raise _elsewhere(page_table, "page_table", dev)
@@ -376,8 +381,8 @@ def _paged(k_cache, v_cache, page_table, q_start, kv_len, tokens: int, max_q: in
             raise ValueError(f"q_start: without it every sequence has one token (got {tokens} tokens, {B} sequences)")
     else:
         q_start = _table(q_start, (B + 1,), torch.int32, "q_start", dev)
-    return cache, _lib.PagedBatch(page_table.data_ptr(), ts[0], width, q_start,
-                                  _table(kv_len, (B,), torch.int32, "kv_len", dev), B, tokens, max_q)
+    return cache, heads, dim, _lib.PagedBatch(page_table.data_ptr(), ts[0], width, q_start,
+                                              _table(kv_len, (B,), torch.int32, "kv_len", dev), B, tokens, max_q)
 
 
 def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -395,8 +400,7 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     behind the last sequence's, and tokens on a page number outside the cache, write nothing.
     `q_out` may be `q`."""
     T, dev = k.shape[0] if isinstance(k, torch.Tensor) and k.dim() == 3 else 0, _device()
-    cache, batch = _paged(k_cache, v_cache, page_table, q_start, kv_len, T, 0, dev)
-    heads, D = cache.heads, cache.dim
+    cache, heads, D, batch = _paged(k_cache, v_cache, page_table, q_start, kv_len, T, 0, dev)
     kt, vt = _tokens(k, "k", heads, D, T, dev), _tokens(v, "v", heads, D, T, dev)
     rot = None if turns is None else _rotation(turns, interleaved, False, magnitude, dev)
     qt = ot = None
@@ -404,10 +408,10 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     if q is not None:
         if rot is None:
             raise ValueError("q: without turns there is nothing to do for the queries")
-        qt = _tokens(q, "q", None, D, T, dev)
+        qt = _tokens(q, "q", 0, D, T, dev)
         Hq = q.shape[1]
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=bf16, device=q.device)
+            q_out = _result(q)
         ot = _tokens(q_out, "q_out", Hq, D, T, dev)
     elif q_out is not None:
         raise ValueError("q_out: there is no q")
@@ -429,12 +433,11 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if max_q is None:
         B = max(kv_len.shape[0], 1) if isinstance(kv_len, torch.Tensor) and kv_len.dim() else 1
         max_q = -(-T // B)
-    cache, batch = _paged(k_cache, v_cache, page_table, q_start, kv_len, T, max_q, dev)
-    D = cache.dim
-    qt = _tokens(q, "q", None, D, T, dev)
+    cache, _, D, batch = _paged(k_cache, v_cache, page_table, q_start, kv_len, T, max_q, dev)
+    qt = _tokens(q, "q", 0, D, T, dev)
     Hq = q.shape[1]
     if out is None:
-        out = torch.empty(q.shape, dtype=bf16, device=q.device)
+        out = _result(q)
     ot = _tokens(out, "out", Hq, D, T, dev)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
