@@ -123,13 +123,13 @@ struct Choice {
   int dp = 0, mt = 0, workers = 0, whole = 0, splits = 0, items = 0;
   size_t workspace() const {
     if (!dp) return 0;
-    const size_t few = mt && workers > 1 && !whole ? 2 * (size_t)workers * pd_part_floats(dp, mt) : 0;
-    const size_t many = splits > 1 ? (size_t)items * splits * pc_part_floats(dp) : 0;
-    return std::max(few, many) * sizeof(float);
+    const size_t few = mt && workers > 1 && !whole ? pd_workspace(dp, mt, workers) : 0;
+    const size_t many = splits > 1 ? (size_t)items * splits * pc_part_floats(dp) * sizeof(float) : 0;
+    return std::max(few, many);
   }
 };
 
-Choice choose(int q_heads, const pk_paged_cache &c, const pk_paged_batch &b) {
+Choice choose(int q_heads, const pk_paged_cache &c, const pk_paged_batch &b, int window) {
   Choice r;
   if (c.dim > 256 || c.dim % 8 != 0) return r;
   const int dp = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
@@ -139,8 +139,12 @@ Choice choose(int q_heads, const pk_paged_cache &c, const pk_paged_batch &b) {
   // a hint of fewer tokens than there are on average is none
   const int64_t most = std::max<int64_t>(b.max_q, ((int64_t)b.tokens + b.sequences - 1) / b.sequences);
   const bool chunks = most * group > PD_ROWS;
-  // every sequence is a chunk where there is one, or where all have the hint's length
-  const bool few = !chunks || !(b.sequences == 1 || (int64_t)b.max_q * b.sequences == b.tokens);
+  // Beside chunks the decode kernel takes the others, but not where every sequence is a chunk
+  // (there is one, or all have the hint's length), nor where no token reaches further than the
+  // chunks' own work goes on (mixed batch of 4 prompts of up to 1531 tokens and 20 single ones, D
+  // 64, the last 1024 keys: 54 us and 17 of the decode kernel and its merge, FIGURE with one kernel).
+  const int64_t reach = window > 0 ? std::min<int64_t>((window + PT_KEYS) / PT_STEP + 2, steps) : steps;
+  const bool few = !chunks || !(b.sequences == 1 || (int64_t)b.max_q * b.sequences == b.tokens || reach <= 32);
   if (chunks) {
     const int64_t items = ((int64_t)b.tokens * group / PC_ROWS + b.sequences) * c.heads;
     const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({slots / items, steps / 8, 32}));
@@ -217,7 +221,7 @@ size_t pk_paged_attention_workspace_size(int q_heads, const pk_paged_cache *cach
   if (!cache || !batch || q_heads <= 0 || cache->heads <= 0 || q_heads % cache->heads != 0 || cache->dim <= 0 ||
       cache->page_size <= 0 || batch->tokens <= 0 || batch->sequences <= 0 || batch->table_width < 0)
     return 0;
-  return choose(q_heads, *cache, *batch).workspace();
+  return choose(q_heads, *cache, *batch, 0).workspace();  // a window takes no more
 }
 
 int launch_paged_attention(const pk_tokens *q, const pk_tokens *out, int q_heads, const pk_paged_cache *cache,
@@ -238,10 +242,10 @@ int launch_paged_attention(const pk_tokens *q, const pk_tokens *out, int q_heads
   g.out = Heads{out->data, 0, out->token, out->head};
   g.q_heads = q_heads;
   g.causal = causal != 0;
-  g.window = window;
+  g.window = window >= g.batch.capacity ? 0 : window;  // (hides nothing)
   g.c2 = scale * 1.4426950408889634f;
   g.group = FastDiv((uint32_t)(q_heads / cache->heads));
-  const Choice c = choose(q_heads, *cache, *batch);
+  const Choice c = choose(q_heads, *cache, *batch, g.window);
   // a scale of 0, infinity or no number has no place in the exponents of the fast kernels
   if (!c.dp || !tile_operands(g) || !(std::fabs(g.c2) > 0.f) || std::isinf(g.c2)) return run_general(g, (hipStream_t)stream);
   if (workspace_bytes < c.workspace() || (c.workspace() && (!workspace || !aligned16(workspace)))) {

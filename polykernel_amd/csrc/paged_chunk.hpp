@@ -5,15 +5,15 @@
 // wave, over steps of 64 keys that the four waves share through LDS.  S^T = K Q^T and
 // O^T = V^T P^T run on v_mfma_f32_32x32x16_bf16 as in the contiguous flash kernel: a lane
 // owns one row and half of the keys, so P never leaves its registers.  P is rounded to
-// bf16 once (half a step, 2^-8 of a weight, its sum kept in fp32): the second product
-// of a low half would be a third of all matrix work.
+// bf16 once (half a step, 2^-8 of a weight; the second product of a low half would be a
+// third of all matrix work), and the fp32 sum is that of the rounded weights, two an
+// instruction, so that what all of them lose in common cancels.
 //
 // Step t + 1's scores are computed while step t's exponentials are, in one run of
 // instructions without a branch (two waves of two workgroups on a SIMD fall into step
 // otherwise, and both wait for the matrix unit and then both for the exponentials).
 //
-// Items of one key head run next to each other on one XCD and share its L2; a sequence's
-// last rows, which see the most keys, come first.  Few items are also cut into `splits`
+// Items of one key head run next to each other on one XCD and share its L2.  Few items are also cut into `splits`
 // runs of keys, whose states paged_chunk_merge_kernel adds in order.
 #pragma once
 
@@ -82,7 +82,10 @@ __device__ __forceinline__ bool find_item(const ChunkArgs &d, int splits, int i,
   it.hk = uniform(in_seq / per_head);
   const int in_head = uniform(in_seq - it.hk * per_head);
   it.split = uniform(in_head / n);
-  it.tile = n - 1 - (in_head - it.split * n);
+  // from the last tile, which sees the most keys, on; where everything runs at once, two
+  // workgroups on a CU, the second half from the first tile on, so that long ones share with short
+  const int x = in_head - it.split * n, turn = total * splits <= 512 ? (n + 1) / 2 : n;
+  it.tile = x < turn ? n - 1 - x : x - turn;
   order = at + it.hk * n + it.tile;
   return order < d.items;
 }
@@ -321,12 +324,13 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
     // weights of scores 2 n and 2 n + 1: three quarters beside the next scores, the rest beside the
     // first products with V, which are those of the other weights
     constexpr int EARLY = 12;
+    const pk_bf16x2 ones = {(__bf16)1.f, (__bf16)1.f};
     auto weights = [&](int n) __attribute__((always_inline)) {
       const int kb = n >> 3, j = 2 * (n & 7);
       const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[kb][j], c2, -mc));
       const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[kb][j + 1], c2, -mc));
-      sum += p0 + p1;
       uint32_t two = pack_bf(p0, p1);
+      sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pk_bf16x2, two), ones, sum, false);
       asm volatile("" : "+v"(two), "+v"(sum));  // here, not where they are used first
       pw[n >> 2][n & 3] = two;
     };

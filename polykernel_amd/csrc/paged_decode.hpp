@@ -33,10 +33,18 @@ constexpr int PD_WAVES = 4, PD_THREADS = PD_WAVES * 64, PD_TILE = PT_KEYS, PD_ST
 
 // Bytes of one workgroup's partial state: 16 MT rows of DP sums, and (maximum, sum).
 constexpr size_t pd_part_floats(int DP, int MT) { return (size_t)16 * MT * (DP + 2); }
+constexpr size_t pd_workspace(int DP, int MT, int workers) {
+  return workers * (2 * pd_part_floats(DP, MT) * sizeof(float) + 32);
+}
 
+// Where a workgroup's part begins inside an item: the item's workgroups and rows, for the merge.
+struct Cut {
+  int first, last, second, q0;  // first < 0: it does not; second: the first's state is its second one
+  int hk, row0, rows, unused;
+};
 struct DecodeArgs {
   AttendArgs a;
-  float *parts;  // two partial states per workgroup
+  float *parts;  // two partial states per workgroup, then a Cut each
   int least;     // steps per workgroup, where there are enough for all
   int most;      // workgroups
   int below;     // rows of a sequence from which on another kernel takes it
@@ -155,8 +163,14 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
   uint8_t *const mine = ring + wid * S::WAVE;  // K slots, then V slots
   const uint32_t mine_at = lds_number(ring) + wid * S::WAVE;
 
+  auto cut = [&](int w) __attribute__((always_inline)) {
+    return reinterpret_cast<Cut *>(d.parts + (size_t)(2 * d.most) * pd_part_floats(DP, MT)) + w;
+  };
   Place at;
-  if (!find_place<ROWS>(d, blockIdx.x, at)) return;
+  if (!find_place<ROWS>(d, blockIdx.x, at)) {
+    if (tid == 0 && d.most > 1 && !d.whole) cut(blockIdx.x)->first = -1;
+    return;
+  }
 
   TileLoader<DP, PAGE16, true> tiles(g);
   int u = at.first, in_seq = at.in_seq, b = at.b;
@@ -398,38 +412,40 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
       }
       __syncthreads();
     }
+    if (first_segment && tid == 0 && d.most > 1 && !d.whole) {
+      Cut c{-1, 0, 0, s.q0, hk, row0, rows, 0};
+      if (st0 > 0) {
+        const int begin = at.first - st0;
+        c.first = at.worker_of(begin);
+        c.last = min(at.worker_of(begin + ln.unit - 1), at.workers - 1);
+        c.second = at.part(c.first) != begin;
+      }
+      *cut(blockIdx.x) = c;
+    }
     u += took;
     in_seq += took;
     first_segment = false;
   }
 }
 
-// Adds the parts of an item that is cut between workgroups w0 to w1: the workgroups of
-// this launch numbered w0 + 1 to w1 share its outputs, 4 dims of a row (a chunk) at a
-// time.  A chunk has as many threads as parts (a power of two up to 16), each on every
-// so-many-th part, and their sums meet in LDS.
+// Adds the parts of an item that is cut between workgroups `first` to `last`: the workgroups
+// of this launch numbered first + 1 to last share its outputs, 4 dims of a row (a chunk) at a
+// time.  A thread reads AT_ONCE parts of a chunk before it adds them; more parts have more
+// threads (a power of two up to 32), whose sums meet in LDS.
 template <int DP, int MT>
 __device__ __forceinline__ void paged_decode_merge_body(const DecodeArgs &d) {
-  constexpr int ROWS = 16 * MT;
+  constexpr int ROWS = 16 * MT, AT_ONCE = 4;
   __shared__ float sum[PD_THREADS][6];
   const AttendArgs &g = d.a;
   const int w = blockIdx.x + 1;
-  Place at;
-  if (!find_place<ROWS>(d, w, at)) return;
-  const Seq s = sequence_at(g.batch, at, at.b);
-  const Line ln = line_of<ROWS>(d, s);
-  const int item = uniform(at.in_seq / ln.unit), st = at.in_seq - item * ln.unit;
-  if (st == 0) return;
-  const int begin = at.first - st;
-  const int w0 = uniform(at.worker_of(begin)), w1 = min(uniform(at.worker_of(begin + ln.unit - 1)), at.workers - 1);
-  const int hk = item / ln.tiles, tile = item - hk * ln.tiles;
-  const int row0 = tile * ROWS, rows = min(ROWS, s.n * (int)g.group.d - row0), D = g.cache.dim;
-  const float c2 = fabsf(g.c2);
   const size_t stride = pd_part_floats(DP, MT);
-  // the first workgroup's part is its second one unless it began with the item
-  const float *p0 = d.parts + (size_t)(2 * w0 + (at.part(w0) == begin ? 0 : 1)) * stride;
-  int groups = 2;
-  while (groups < 16 && groups < w1 - w0 + 1) groups *= 2;
+  const Cut cut = reinterpret_cast<const Cut *>(d.parts + (size_t)(2 * d.most) * stride)[w];
+  const int w0 = cut.first, w1 = cut.last, rows = cut.rows, D = g.cache.dim;
+  if (w0 < 0) return;
+  const float c2 = fabsf(g.c2);
+  const float *p0 = d.parts + (size_t)(2 * w0 + cut.second) * stride;
+  int groups = 1;
+  while (groups < 32 && AT_ONCE * groups < w1 - w0 + 1) groups *= 2;
   const int lanes = PD_THREADS / groups, lane = threadIdx.x & (lanes - 1), grp = threadIdx.x / lanes;
   const int cpr = D / 4, chunks = rows * cpr;
   auto weight = [&](float m, float M) __attribute__((always_inline)) {
@@ -439,35 +455,55 @@ __device__ __forceinline__ void paged_decode_merge_body(const DecodeArgs &d) {
     const int c = min(c0 + lane, chunks - 1), r = c / cpr, dd = 4 * (c - r * cpr);
     float M = -INFINITY, L = 0.f;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int k = w0 + grp; k <= w1; k += groups) {
-      const float *p = k == w0 ? p0 : d.parts + (size_t)(2 * k) * stride;
-      const float m = p[(size_t)ROWS * DP + 2 * r], l = p[(size_t)ROWS * DP + 2 * r + 1];
-      const f32x4 o = *reinterpret_cast<const f32x4 *>(p + (size_t)r * DP + dd);
-      const float M2 = fmaxf(M, m), a = weight(M, M2), f = weight(m, M2);
-      L = L * a + l * f;
-      v = v * a + o * f;
+    for (int k0 = w0 + grp; k0 <= w1; k0 += AT_ONCE * groups) {
+      float m[AT_ONCE], l[AT_ONCE];
+      f32x4 o[AT_ONCE];
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const int k = min(k0 + i * groups, w1);
+        const float *p = k == w0 ? p0 : d.parts + (size_t)(2 * k) * stride;
+        const float2 ml = *reinterpret_cast<const float2 *>(p + (size_t)ROWS * DP + 2 * r);
+        o[i] = *reinterpret_cast<const f32x4 *>(p + (size_t)r * DP + dd);
+        m[i] = k0 + i * groups <= w1 ? ml.x : -INFINITY;
+        l[i] = ml.y;
+      }
+      float M2 = M;
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) M2 = fmaxf(M2, m[i]);
+      const float a = weight(M, M2);
+      L *= a;
+      v *= a;
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const float f = weight(m[i], M2);
+        L += l[i] * f;
+        v += o[i] * f;
+      }
       M = M2;
     }
-    float *x = sum[threadIdx.x];
-    x[0] = M, x[1] = L, x[2] = v[0], x[3] = v[1], x[4] = v[2], x[5] = v[3];
-    __syncthreads();
-    if (grp == 0 && c0 + lane < chunks) {
-      const int n = min(groups, w1 - w0 + 1);
-      for (int k = 1; k < n; ++k) M = fmaxf(M, sum[k * lanes + lane][0]);
-      L = 0.f;
-      v = f32x4{0.f, 0.f, 0.f, 0.f};
-      for (int k = 0; k < n; ++k) {
-        const float *y = sum[k * lanes + lane];
-        const float f = weight(y[0], M);
-        L += y[1] * f;
-        v += f32x4{y[2], y[3], y[4], y[5]} * f;
+    if (groups > 1) {
+      float *x = sum[threadIdx.x];
+      x[0] = M, x[1] = L, x[2] = v[0], x[3] = v[1], x[4] = v[2], x[5] = v[3];
+      __syncthreads();
+      if (grp == 0) {
+        for (int k = 1; k < groups; ++k) M = fmaxf(M, sum[k * lanes + lane][0]);
+        L = 0.f;
+        v = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < groups; ++k) {
+          const float *y = sum[k * lanes + lane];
+          const float f = weight(y[0], M);
+          L += y[1] * f;
+          v += f32x4{y[2], y[3], y[4], y[5]} * f;
+        }
       }
+      __syncthreads();
+    }
+    if (grp == 0 && c0 + lane < chunks) {
       const float inv = L == 0.f ? 0.f : 1.f / L;
-      const int i = (int)g.group.div(row0 + r), h = hk * (int)g.group.d + row0 + r - i * (int)g.group.d;
-      *reinterpret_cast<att::u32x2 *>(g.out.data + (int64_t)(s.q0 + i) * g.out.token + h * g.out.head + dd) =
+      const int i = (int)g.group.div(cut.row0 + r), h = cut.hk * (int)g.group.d + cut.row0 + r - i * (int)g.group.d;
+      *reinterpret_cast<att::u32x2 *>(g.out.data + (int64_t)(cut.q0 + i) * g.out.token + h * g.out.head + dd) =
           att::u32x2{pack_bf(v[0] * inv, v[1] * inv), pack_bf(v[2] * inv, v[3] * inv)};
     }
-    __syncthreads();
   }
 }
 

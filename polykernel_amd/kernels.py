@@ -357,32 +357,47 @@ def _tokens(t: torch.Tensor, name: str, heads: int, dim: int, tokens: int, dev: 
     return _lib.Tokens(t.data_ptr(), strides[0], strides[1])
 
 
-def _paged(k_cache, v_cache, page_table, q_start, kv_len, tokens: int, max_q: int, dev: int):
-    ks, vs = _heads(k_cache, 4, "k_cache", dev), _heads(v_cache, 4, "v_cache", dev)
-    shape = k_cache.shape
-    if shape != v_cache.shape:
-        raise ValueError(f"k_cache and v_cache must have the same shape, got {tuple(shape)}, {tuple(v_cache.shape)}")
-    pages, heads, rows, dim = shape
-    cache = _lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), *ks[:3], *vs[:3], pages, rows, heads, dim)
+def _refuse_paged(k_cache, v_cache, page_table, kv_len, dev: int) -> None:
+    """Says what is wrong with the tables or caches of a paged call."""
+    _heads(k_cache, 4, "k_cache", dev), _heads(v_cache, 4, "v_cache", dev)
+    if k_cache.shape != v_cache.shape:
+        raise ValueError("k_cache and v_cache must have the same shape, got "
+                         f"{tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
     if not isinstance(kv_len, torch.Tensor) or kv_len.dim() != 1:
         raise ValueError("kv_len: expected an int32 tensor [sequences]")
     B = kv_len.shape[0]
+    _table(kv_len, (B,), torch.int32, "kv_len", dev)
     if not isinstance(page_table, torch.Tensor) or page_table.dim() != 2 or page_table.shape[0] != B:
         raise ValueError(f"page_table: expected an int32 tensor [{B}, pages of a sequence]")
-    if page_table.dtype is not torch.int32:
+    if page_table.dtype != torch.int32:
         raise TypeError(f"page_table: expected {torch.int32}, got {page_table.dtype}")
     if page_table.get_device() != dev:
         raise _elsewhere(page_table, "page_table", dev)
-    ts, width = page_table.stride(), page_table.shape[1]
-    if ts[1] != 1 and width > 1:
-        raise ValueError("page_table: the pages of a sequence must be contiguous")
-    if q_start is None:
-        if tokens != B:
-            raise ValueError(f"q_start: without it every sequence has one token (got {tokens} tokens, {B} sequences)")
-    else:
+    raise ValueError("page_table: the pages of a sequence must be contiguous")
+
+
+def _paged(k_cache, v_cache, page_table, q_start, kv_len, tokens: int, max_q: int, dev: int):
+    """(cache, heads, dim, batch) for the C entry points, once everything is as it has to be: one
+    condition, since a step's call takes no longer than its checks."""
+    try:
+        (k0, k1, k2, k3), (v0, v1, v2, v3) = k_cache.stride(), v_cache.stride()
+        pages, heads, rows, dim = shape = k_cache.shape
+        B, width = page_table.shape
+        t0, t1 = page_table.stride()
+        fine = (shape == v_cache.shape and ((k3 == 1 and v3 == 1) or dim <= 1) and (t1 == 1 or width <= 1)
+                and k_cache.dtype is bf16 and v_cache.dtype is bf16 and page_table.dtype is kv_len.dtype is torch.int32
+                and kv_len.shape == (B,) and kv_len.is_contiguous()
+                and k_cache.get_device() == v_cache.get_device() == page_table.get_device() == kv_len.get_device() == dev)
+    except (AttributeError, ValueError):
+        fine = False
+    if not fine:
+        _refuse_paged(k_cache, v_cache, page_table, kv_len, dev)
+    if q_start is not None:
         q_start = _table(q_start, (B + 1,), torch.int32, "q_start", dev)
-    return cache, heads, dim, _lib.PagedBatch(page_table.data_ptr(), ts[0], width, q_start,
-                                              _table(kv_len, (B,), torch.int32, "kv_len", dev), B, tokens, max_q)
+    elif tokens != B:
+        raise ValueError(f"q_start: without it every sequence has one token (got {tokens} tokens, {B} sequences)")
+    return (_lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), k0, k1, k2, v0, v1, v2, pages, rows, heads, dim), heads,
+            dim, _lib.PagedBatch(page_table.data_ptr(), t0, width, q_start, kv_len.data_ptr(), B, tokens, max_q))
 
 
 def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -412,7 +427,9 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
         Hq = q.shape[1]
         if q_out is None:
             q_out = _result(q)
-        ot = _tokens(q_out, "q_out", Hq, D, T, dev)
+            ot = _lib.Tokens(q_out.data_ptr(), Hq * D, D)
+        else:
+            ot = _tokens(q_out, "q_out", Hq, D, T, dev)
     elif q_out is not None:
         raise ValueError("q_out: there is no q")
     check(_lib.load().launch_paged_kv_append(kt, vt, qt, ot, Hq, cache, batch, rot, _stream()), "launch_paged_kv_append")
@@ -438,7 +455,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     Hq = q.shape[1]
     if out is None:
         out = _result(q)
-    ot = _tokens(out, "out", Hq, D, T, dev)
+        ot = _lib.Tokens(out.data_ptr(), Hq * D, D)
+    else:
+        ot = _tokens(out, "out", Hq, D, T, dev)
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     lib = _lib.load()
