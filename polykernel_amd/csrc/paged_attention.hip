@@ -103,7 +103,7 @@ __global__ __launch_bounds__(PD_THREADS) void paged_decode_merge_kernel(DecodeAr
   paged_decode_merge_body<DP, MT>(d);
 }
 template <int DP, bool PAGE16>
-__global__ __launch_bounds__(PC_THREADS, DP == 256 ? 1 : DP == 64 ? 3 : 2) void paged_chunk_kernel(ChunkArgs d) {
+__global__ __launch_bounds__(PC_THREADS, DP == 256 ? 1 : DP == 64 ? 4 : 2) void paged_chunk_kernel(ChunkArgs d) {
   paged_chunk_body<DP, PAGE16>(d);
 }
 template <int DP>

@@ -100,6 +100,7 @@ __device__ __forceinline__ void lds_barrier() {
 template <int DP>
 struct ChunkShape {
   static constexpr int TB = PC_STEP * DP * 2, SL = 2;  // bytes of a step, slots of a ring
+  static constexpr bool PIPE = DP != 64;                     // the next step's scores beside this one's weights
   static constexpr int OS = DP * 2 + 16;                             // row stride of a wave's rows on their way out
   static constexpr int LDS = 2 * SL * TB;
   static_assert(PC_ROWS * OS <= LDS, "the outputs pass through the rings");
@@ -303,10 +304,18 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
     lds_barrier();  // and every wave's; nobody reads what the next loads overwrite
     uint8_t *const vs = ring + (SL + sl) * TB;
     const int key = kfirst + t * PC_STEP;
+    if constexpr (S::PIPE) {
+      issue_v(t + 1, next);
+    } else {
+      issue_k(t + 1, next);
+      issue_v(t + 1, next);
+      scores(sl, sc, [](int) {});
+      top = maximum(sc);
+      mask(t, sl);
+    }
     // the same for every wave: whether some row of the item has a hidden key in this step
     const bool mixed = key < t1 || key + PC_STEP > t0 || !whole;
-    issue_v(t + 1, next);
-    issue_k(t + 2, sl);
+    if constexpr (S::PIPE) issue_k(t + 2, sl);
 
     // the maximum in the exponent follows once it is 2^8 behind
     if (__any((top - m_run) * c2 > 8.f)) {
@@ -323,7 +332,7 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
     float sum = 0.f;
     // weights of scores 2 n and 2 n + 1: three quarters beside the next scores, the rest beside the
     // first products with V, which are those of the other weights
-    constexpr int EARLY = 12;
+    constexpr int EARLY = S::PIPE ? 12 : 16;
     const pk_bf16x2 ones = {(__bf16)1.f, (__bf16)1.f};
     auto weights = [&](int n) __attribute__((always_inline)) {
       const int kb = n >> 3, j = 2 * (n & 7);
@@ -334,10 +343,15 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
       asm volatile("" : "+v"(two), "+v"(sum));  // here, not where they are used first
       pw[n >> 2][n & 3] = two;
     };
-    scores(next, nx, [&](int i) __attribute__((always_inline)) {
+    if constexpr (S::PIPE) {
+      scores(next, nx, [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-      for (int n = i * EARLY / NA; n < (i + 1) * EARLY / NA; ++n) weights(n);
-    });
+        for (int n = i * EARLY / NA; n < (i + 1) * EARLY / NA; ++n) weights(n);
+      });
+    } else {
+#pragma unroll
+      for (int n = 0; n < EARLY; ++n) weights(n);
+    }
 
     if (mixed) {
       pk_u16x2 most = {0, 0};
@@ -364,7 +378,7 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
     }
     {
       bf16x8 f[NB];
-      top = nx[0][0];
+      if constexpr (S::PIPE) top = nx[0][0];
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) f[i] = v_fragment(sl, i);
       __builtin_amdgcn_sched_barrier(0);
@@ -376,29 +390,34 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
           constexpr int ON = 3 * DB;  // products with the early weights
 #pragma unroll
           for (int n = EARLY + j * (16 - EARLY) / ON; n < min(16, EARLY + (j + 1) * (16 - EARLY) / ON); ++n) weights(n);
+          if constexpr (S::PIPE)
 #pragma unroll
-          for (int n = j * 32 / NB; n < (j + 1) * 32 / NB; ++n) top = fmaxf(top, nx[n >> 4][n & 15]);
+            for (int n = j * 32 / NB; n < (j + 1) * 32 / NB; ++n) top = fmaxf(top, nx[n >> 4][n & 15]);
         }
 #pragma unroll
         for (int j = i + AHEAD; j < min(NB, i + AHEAD + 2); ++j) f[j] = v_fragment(sl, j);
         __builtin_amdgcn_sched_barrier(0);
       }
       l_run += sum;
-      top = xor32_max(top);
     }
-    sc[0] = nx[0];
-    sc[1] = nx[1];
-    mask(t + 1, next);
+    if constexpr (S::PIPE) {
+      top = xor32_max(top);
+      sc[0] = nx[0];
+      sc[1] = nx[1];
+      mask(t + 1, next);
+    }
   };
 
   issue_k(0, 0);
   issue_v(0, 0);
-  issue_k(1, 1);
-  vm_wait<2 * NI>();
-  lds_barrier();
-  scores(0, sc, [](int) {});
-  top = maximum(sc);
-  mask(0, 0);
+  if constexpr (S::PIPE) {
+    issue_k(1, 1);
+    vm_wait<2 * NI>();
+    lds_barrier();
+    scores(0, sc, [](int) {});
+    top = maximum(sc);
+    mask(0, 0);
+  }
   int t = 0;
 #pragma unroll 1
   for (; t + 1 < nst; t += 2) {
