@@ -275,6 +275,18 @@ PK_API int launch_paged_attention(const pk_tokens *q, const pk_tokens *out, int 
                                   const pk_paged_batch *batch, float scale, int causal, int window, void *workspace,
                                   size_t workspace_bytes, void *stream);
 
+/* Test hook: how launch_paged_attention takes a call with 16-byte aligned operands
+ * and strides (no device is needed).  dim 0: the general kernel.  step_rows > 0: the
+ * step kernel, with that many rows (tokens x query heads of a group) per item and
+ * `workgroups`, which cut items between them unless `whole`; splits > 0: the chunk
+ * kernel, `items` items at most, each in that many runs of keys.  With both, sequences
+ * of up to 64 rows are the step kernel's. */
+typedef struct pk_paged_plan {
+  int dim, step_rows, workgroups, whole, splits, items;
+} pk_paged_plan;
+PK_API int pk_paged_attention_plan(int q_heads, const pk_paged_cache *cache, const pk_paged_batch *batch, int window,
+                                   pk_paged_plan *out);
+
 /* Config-2 MLP block: y = add(bias(matmul(gelu(bias(matmul(rmsnorm(x, gamma),
  * W1), b1)), W2), b2), x).  x [M,d], W1 [d,F], W2 [F,d].  `workspace` must
  * hold pk_mlp_block_workspace_size(M, d, F) bytes (the normalised rows and the

@@ -80,6 +80,13 @@ class PagedBatch(C.Structure):
                 ("max_q", C.c_int)]
 
 
+class PagedPlan(C.Structure):
+    """struct pk_paged_plan: the kernels of a paged attention call."""
+
+    _fields_ = [("dim", C.c_int), ("step_rows", C.c_int), ("workgroups", C.c_int), ("whole", C.c_int),
+                ("splits", C.c_int), ("items", C.c_int)]
+
+
 ROTARY_SCALINGS = ("none", "linear", "base", "bands", "ramp")
 
 PLAN_TILE, PLAN_STREAM, PLAN_RING, PLAN_ODD, PLAN_RAGGED = range(5)
@@ -128,6 +135,7 @@ SIGNATURES = {
     "launch_paged_kv_append": (I, [C.POINTER(Tokens), C.POINTER(Tokens), C.POINTER(Tokens), C.POINTER(Tokens), I,
                                    C.POINTER(PagedCache), C.POINTER(PagedBatch), C.POINTER(Rotary), P]),
     "pk_paged_attention_workspace_size": (SZ, [I, C.POINTER(PagedCache), C.POINTER(PagedBatch)]),
+    "pk_paged_attention_plan": (I, [I, C.POINTER(PagedCache), C.POINTER(PagedBatch), I, C.POINTER(PagedPlan)]),
     "launch_paged_attention": (I, [C.POINTER(Tokens), C.POINTER(Tokens), I, C.POINTER(PagedCache),
                                    C.POINTER(PagedBatch), F, I, I, P, SZ, P]),
     "pk_mlp_block_workspace_size": (SZ, [I, I, I]),

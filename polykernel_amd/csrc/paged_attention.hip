@@ -102,9 +102,9 @@ template <int DP, int MT>
 __global__ __launch_bounds__(PD_THREADS) void paged_decode_merge_kernel(DecodeArgs d) {
   paged_decode_merge_body<DP, MT>(d);
 }
-template <int DP, bool PAGE16>
+template <int DP, int DC, bool PAGE16>
 __global__ __launch_bounds__(PC_THREADS, DP == 256 ? 1 : DP == 64 ? 4 : 2) void paged_chunk_kernel(ChunkArgs d) {
-  paged_chunk_body<DP, PAGE16>(d);
+  paged_chunk_body<DP, DC, PAGE16>(d);
 }
 template <int DP>
 __global__ __launch_bounds__(PC_THREADS) void paged_chunk_merge_kernel(ChunkArgs d) {
@@ -185,6 +185,18 @@ int run_decode_as(const DecodeArgs &d, hipStream_t st) {
   }
   return PK_OK;
 }
+template <int DP, int DC>
+int run_chunk_as(const ChunkArgs &d, hipStream_t st) {
+  const unsigned blocks = (unsigned)d.items * d.splits;
+  if (d.a.cache.page.d % PT_KEYS == 0) paged_chunk_kernel<DP, DC, true><<<blocks, PC_THREADS, 0, st>>>(d);
+  else paged_chunk_kernel<DP, DC, false><<<blocks, PC_THREADS, 0, st>>>(d);
+  PK_LAUNCH_CHECK("paged_chunk_kernel");
+  if (d.splits > 1) {
+    paged_chunk_merge_kernel<DP><<<dim3(d.items, PC_ROWS / PC_MERGE_ROWS), PC_THREADS, 0, st>>>(d);
+    PK_LAUNCH_CHECK("paged_chunk_merge_kernel");
+  }
+  return PK_OK;
+}
 template <int DP>
 int run_as(const AttendArgs &g, const Choice &c, float *workspace, hipStream_t st) {
   if (c.mt) {
@@ -197,13 +209,10 @@ int run_as(const AttendArgs &g, const Choice &c, float *workspace, hipStream_t s
   }
   if (c.splits) {
     const ChunkArgs d{g, workspace, c.items, c.splits, c.mt ? PD_ROWS : 0};
-    if (g.cache.page.d % PT_KEYS == 0) paged_chunk_kernel<DP, true><<<c.items * c.splits, PC_THREADS, 0, st>>>(d);
-    else paged_chunk_kernel<DP, false><<<c.items * c.splits, PC_THREADS, 0, st>>>(d);
-    PK_LAUNCH_CHECK("paged_chunk_kernel");
-    if (c.splits > 1) {
-      paged_chunk_merge_kernel<DP><<<dim3(c.items, PC_ROWS / PC_MERGE_ROWS), PC_THREADS, 0, st>>>(d);
-      PK_LAUNCH_CHECK("paged_chunk_merge_kernel");
-    }
+    // three quarters of the dims are products enough for head dims up to there
+    if constexpr (DP > 64)
+      if (g.cache.dim <= DP / 4 * 3) return run_chunk_as<DP, DP / 4 * 3>(d, st);
+    return run_chunk_as<DP, DP>(d, st);
   }
   return PK_OK;
 }
@@ -216,6 +225,19 @@ using namespace pk;
 using namespace pk::paged;
 
 extern "C" {
+
+int pk_paged_attention_plan(int q_heads, const pk_paged_cache *cache, const pk_paged_batch *batch, int window,
+                            pk_paged_plan *out) {
+  const char *who = "pk_paged_attention_plan";
+  Cache c;
+  Batch b;
+  if (int rc = check_cache(who, cache, &c)) return rc;
+  if (int rc = check_batch(who, batch, cache, &b)) return rc;
+  PK_CHECK_ARG(out && q_heads > 0 && q_heads % cache->heads == 0 && window >= 0 && batch->sequences > 0, "%s: invalid argument", who);
+  const Choice r = choose(q_heads, *cache, *batch, window >= b.capacity ? 0 : window);
+  *out = pk_paged_plan{r.dp, 16 * r.mt, r.workers, r.whole, r.splits, r.items};
+  return PK_OK;
+}
 
 size_t pk_paged_attention_workspace_size(int q_heads, const pk_paged_cache *cache, const pk_paged_batch *batch) {
   if (!cache || !batch || q_heads <= 0 || cache->heads <= 0 || q_heads % cache->heads != 0 || cache->dim <= 0 ||

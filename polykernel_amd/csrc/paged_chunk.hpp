@@ -106,11 +106,13 @@ struct ChunkShape {
   static_assert(PC_ROWS * OS <= LDS, "the outputs pass through the rings");
 };
 
-template <int DP, bool PAGE16>
+// DP: dims of a row in LDS; DC: dims that the products take (head dims up to DC).
+template <int DP, int DC, bool PAGE16>
 __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
   using S = ChunkShape<DP>;
   using Tiles = TileLoader<DP, PAGE16, false>;
-  constexpr int CH = DP / 8, TB = S::TB, SL = S::SL, NI = Tiles::NI, DS = DP / 16, DB = DP / 32, RB = DP * 2;
+  constexpr int CH = DP / 8, TB = S::TB, SL = S::SL, NI = Tiles::NI, DS = DC / 16, DB = DC / 32, RB = DP * 2;
+  static_assert(DC <= DP && DC % 32 == 0, "dims");
   constexpr int KO = DS < 8 ? DS : 8, VO = DB < 4 ? DB : 4;  // lane offsets; dims from 128 on lie 256 bytes further
   __shared__ __attribute__((aligned(1024))) uint8_t ring[S::LDS];
   __shared__ __attribute__((aligned(8))) uint16_t there_s[SL][PC_WAVES];

@@ -327,6 +327,44 @@ def test_attention_rows_first_and_hints(pk, qs, kvs, Hq, Hkv, D, P):
     assert len(outs) == 5
 
 
+def plan(qs, kvs, Hq, Hkv, D, P, max_q, window=0):
+    from tests.test_paged_host import attention_plan
+
+    return attention_plan(q_heads=Hq, heads=Hkv, dim=D, page_size=P, table_width=-(-max(kvs) // P), tokens=sum(qs),
+                          sequences=len(qs), max_q=max_q, window=window)
+
+
+@pytest.mark.parametrize("window", [0, 2200])
+@pytest.mark.parametrize("Hq,Hkv,D,P", [(8, 2, 128, 16), (4, 4, 64, 32), (6, 1, 80, 48), (4, 2, 256, 64), (16, 2, 96, 8),
+                                        (3, 1, 192, 16)])
+def test_chunks_beside_single_tokens(pk, Hq, Hkv, D, P, window):
+    """Both kernels in one call: sequences of up to 64 rows by one, the others by the other."""
+    qs, kvs = [200, 1, 3, 64 // (Hq // Hkv), 0, 64 // (Hq // Hkv) + 1, 1], [2600, 2303, 3, 1000, 7, 100, 40]
+    got = plan(qs, kvs, Hq, Hkv, D, P, max(qs), window)
+    assert got.step_rows > 0 and got.splits > 0
+    run(pk, qs, kvs, Hq, Hkv, D, P, std=2.0, max_q=max(qs), window=window, behind=1)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,P", [(8, 2, 128, 16), (2, 1, 64, 8), (40, 1, 64, 16), (24, 1, 128, 16), (5, 1, 256, 16)])
+def test_many_sequences_cut_between_workgroups(pk, Hq, Hkv, D, P):
+    """More sequences than lanes of a wave, of very different lengths, two without new tokens."""
+    qs = [0 if i in (0, 99) else 1 + (i % 7 == 0) for i in range(150)]
+    kvs = [max(1, (i * 977) % 1400) + 2 for i in range(150)]
+    kvs[31] = 9000
+    got = plan(qs, kvs, Hq, Hkv, D, P, 1)
+    assert got.step_rows > 0 and not got.whole and got.workgroups > 1  # (80 rows of two tokens are a chunk)
+    run(pk, qs, kvs, Hq, Hkv, D, P, std=2.0, max_q=1)
+
+
+@pytest.mark.parametrize("D,P", [(64, 16), (128, 32), (96, 8), (256, 16)])
+@pytest.mark.parametrize("q,kv", [(100, 3000), (33, 5000), (300, 1500)])
+def test_chunks_cut_along_their_keys(pk, q, kv, D, P):
+    got = plan([q], [kv], 4, 1, D, P, q)
+    assert got.splits > 1 and got.step_rows == 0
+    run(pk, [q], [kv], 4, 1, D, P, std=2.0, max_q=q)
+    run(pk, [q], [kv], 4, 1, D, P, std=2.0, max_q=q, window=700)
+
+
 @pytest.mark.parametrize("window", [1, 2, 16, 63, 64, 200, 100000])
 @pytest.mark.parametrize("qs,kvs,Hq,Hkv,D,P", [([1, 1, 1], [1, 70, 1000], 8, 2, 128, 16),
                                                ([5, 2], [300, 40], 8, 2, 64, 32),

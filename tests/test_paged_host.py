@@ -198,3 +198,54 @@ def i32(*shape):
 def test_front_end_refuses(call, error, word):
     with pytest.raises(error, match=word):
         call()
+
+
+# ---- which kernels take a call ----------------------------------------------------------
+def attention_plan(q_heads=32, heads=8, dim=128, page_size=16, table_width=64, tokens=1, sequences=1, max_q=1, window=0):
+    out = _lib.PagedPlan()
+    cache = paged_cache(heads=heads, dim=dim, page_size=page_size, pages=1000)
+    batch = paged_batch(table_width=table_width, tokens=tokens, sequences=sequences, max_q=max_q)
+    _lib.check(_lib.load().pk_paged_attention_plan(q_heads, cache, batch, window, out), "pk_paged_attention_plan")
+    size = _lib.load().pk_paged_attention_workspace_size(q_heads, cache, batch)
+    if not out.dim or (out.splits <= 1 and (out.whole or out.workgroups <= 1)):
+        assert size == 0 or window
+    return out
+
+
+def test_plans():
+    p = attention_plan()  # a step on up to 1024 keys
+    assert (p.dim, p.step_rows, p.whole, p.splits) == (128, 16, 0, 0) and 1 < p.workgroups <= 512
+    p = attention_plan(table_width=20)  # up to 320 keys: items are not cut, and nothing merged
+    assert p.whole == 1 and p.workgroups == 8 and p.splits == 0
+    assert attention_plan(q_heads=256, heads=8).step_rows == 32
+    assert attention_plan(q_heads=512, heads=8).step_rows == 64
+    assert attention_plan(q_heads=512, heads=8, dim=256).step_rows == 32
+    p = attention_plan(tokens=2048, max_q=2048, table_width=512)
+    assert p.step_rows == 0 and p.splits == 1 and p.items == (2048 * 4 // 128 + 1) * 8
+    assert attention_plan(tokens=64, max_q=64, table_width=512).splits > 1
+    mixed = dict(tokens=600, sequences=40, max_q=500)
+    p = attention_plan(**mixed, table_width=512)
+    assert p.step_rows == 16 and p.splits >= 1
+    assert attention_plan(**mixed, table_width=512, window=512).step_rows == 0  # nobody reaches far
+    assert attention_plan(**mixed, table_width=100).step_rows == 0
+    assert attention_plan(tokens=600, sequences=4, max_q=150, table_width=512).step_rows == 0  # all as long as the hint
+    for general in (dict(dim=20), dict(dim=320), dict(dim=1024)):
+        assert attention_plan(**general).dim == 0
+    # a line of steps that a 32-bit place cannot hold goes to the general kernel
+    p = attention_plan(tokens=1 << 20, sequences=1 << 20, table_width=1 << 20, q_heads=64, heads=64)
+    assert p.dim == 0
+
+
+def test_workspace_refused():
+    c, b = paged_cache(k_page=2048, heads=2, dim=64), paged_batch(table_width=100)
+    need = _lib.load().pk_paged_attention_workspace_size(4, c, b)
+    assert need > 0
+    for ws, room in ((None, 0), (None, need), (FAKE, need - 1), (FAKE + 8, need)):
+        assert attend_call(cache=c, batch=b, ws=ws, ws_bytes=room) == _lib.PK_ERR_WORKSPACE
+        assert "workspace" in _lib.last_error()
+
+
+@pytest.mark.parametrize("kw", [dict(q_heads=3), dict(q_heads=0), dict(window=-1), dict(sequences=0)])
+def test_plan_refused(kw):
+    with pytest.raises(_lib.PolyKernelError, match="pk_paged_attention_plan"):
+        attention_plan(**kw)
