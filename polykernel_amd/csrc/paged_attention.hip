@@ -95,7 +95,7 @@ int run_general(const AttendArgs &g, hipStream_t st) {
 
 // ---- the fast kernels (paged_decode.hpp, paged_chunk.hpp) ------------------------
 template <int DP, int MT, bool PAGE16>
-__global__ __launch_bounds__(PD_THREADS, DP == 256 ? 1 : 2) void paged_decode_kernel(DecodeArgs d) {
+__global__ __launch_bounds__(PD_THREADS, (DecodeShape<DP, MT>::GROUPS)) void paged_decode_kernel(DecodeArgs d) {
   paged_decode_body<DP, MT, PAGE16>(d);
 }
 template <int DP, int MT>
@@ -111,7 +111,14 @@ __global__ __launch_bounds__(PC_THREADS) void paged_chunk_merge_kernel(ChunkArgs
   paged_chunk_merge_body<DP>(d);
 }
 
-constexpr int PD_LEAST = 4;   // steps of a workgroup
+constexpr int PD_LEAST = 1;   // steps of a workgroup
+// Workgroups of the step kernel on a CU.
+constexpr int step_groups(int dp, int mt) {
+  return dp == 64    ? mt == 1 ? DecodeShape<64, 1>::GROUPS : mt == 2 ? DecodeShape<64, 2>::GROUPS : DecodeShape<64, 4>::GROUPS
+         : dp == 128 ? mt == 1 ? DecodeShape<128, 1>::GROUPS : mt == 2 ? DecodeShape<128, 2>::GROUPS : DecodeShape<128, 4>::GROUPS
+         : mt == 1   ? DecodeShape<256, 1>::GROUPS
+                     : DecodeShape<256, 2>::GROUPS;
+}
 constexpr int PD_ROWS = 64;   // rows (tokens x heads of a group) of a sequence up to which it is not a chunk
 
 // How a call runs: head dims padded to `dp` (0: by the general kernel); sequences of up to
@@ -133,7 +140,7 @@ Choice choose(int q_heads, const pk_paged_cache &c, const pk_paged_batch &b, int
   Choice r;
   if (c.dim > 256 || c.dim % 8 != 0) return r;
   const int dp = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
-  const int64_t slots = dp == 256 ? 256 : 512;  // workgroups that run at once
+  const int64_t slots = dp == 256 ? 256 : 512;  // chunk workgroups that run at once
   const int64_t group = q_heads / c.heads;
   const int64_t steps = (int64_t)b.table_width * c.page_size / PT_STEP + 2;  // of an item, at most
   // a hint of fewer tokens than there are on average is none
@@ -159,7 +166,7 @@ Choice choose(int q_heads, const pk_paged_cache &c, const pk_paged_batch &b, int
     const int64_t items = ((int64_t)b.tokens * group / (16 * r.mt) + b.sequences) * c.heads;
     if (items > INT32_MAX / steps) return r;  // a line of 2^31 steps or more: the general kernel
     r.whole = steps <= 8;
-    r.workers = (int)std::max<int64_t>(1, std::min(slots, r.whole ? items : items * steps / PD_LEAST));
+    r.workers = (int)std::max<int64_t>(1, std::min<int64_t>(256 * step_groups(dp, r.mt), r.whole ? items : items * steps / PD_LEAST));
   }
   r.dp = dp;
   return r;

@@ -10,9 +10,11 @@
 // by transposing reads.  So P stays in registers; P is split into two bf16 halves
 // (2^-17 relative), which costs nothing under the memory time.
 //
-// Memory: every wave has a ring of its own of SL tiles of 16 keys in LDS, filled by
+// Memory: every wave has rings of its own of SL tiles of 16 keys in LDS, filled by
 // direct-to-LDS loads (16 bytes a lane, chunks swizzled at the source), with no
-// barrier in the loop.  A tile of a page size that is a multiple of 16 lies in one
+// barrier in the loop; a tile's keys make room for those SL tiles on as soon as they
+// are read, its values likewise.  Short rings and many workgroups on a CU keep as many
+// bytes in flight as long rings and few, and hide each other's beginnings and ends.  A tile of a page size that is a multiple of 16 lies in one
 // page: its base address is a buffer resource whose length ends the tile at the last
 // key, so rows behind it read as zero and stale pages never reach a product.  Other
 // page sizes look up a page per row and point rows that are not there at zeros.
@@ -133,19 +135,19 @@ __device__ __forceinline__ bool find_place(const DecodeArgs &d, int w, Place &p)
   }
 }
 
-template <int DP>
+template <int DP, int MT>
 struct DecodeShape {
   static constexpr int NI = TileLoader<DP, true, true>::NI, TB = TileLoader<DP, true, true>::BYTES;
-  static constexpr int SL = DP == 64 ? 4 : 2;
-  static constexpr int WAVE = 2 * SL * TB;  // ring of a wave
-  static constexpr int PS = DP + 4;         // row stride of a state in LDS, floats
-  static constexpr int STATE = 16 * PS * 4;  // a wave's 16 rows of sums, then its (maximum, sum) of up to 64 rows
-  static_assert(STATE + 64 * 8 <= WAVE, "a wave's state lies in its ring");
+  static constexpr int SL = DP == 64 ? 2 : 1;  // tiles of a ring
+  static constexpr int PS = DP + 4;            // row stride of a state in LDS, floats
+  static constexpr int STATE = 16 * PS * 4;    // a wave's 16 rows of sums, then its (maximum, sum) of all rows
+  static constexpr int WAVE = 2 * SL * TB > STATE + 128 * MT ? 2 * SL * TB : STATE + 128 * MT;  // its rings, later its state
+  static constexpr int GROUPS = MT == 1 ? (DP == 256 ? 2 : 4) : DP == 256 ? 1 : MT == 2 ? 3 : 2;  // workgroups on a CU
 };
 
 template <int DP, int MT, bool PAGE16>
 __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
-  using S = DecodeShape<DP>;
+  using S = DecodeShape<DP, MT>;
   constexpr int CH = DP / 8, NI = S::NI, TB = S::TB, SL = S::SL, PS = S::PS;
   constexpr int ROWS = 16 * MT, KS = DP / 32, DB = DP / 16;
   // many query fragments are read from LDS at each tile (the waves share them), few stay in registers
@@ -227,10 +229,8 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
     }
     const float c2 = fabsf(g.c2);
 
-    auto issue = [&](int t) __attribute__((always_inline)) {
-      tiles.issue_k(g, t, mine_at + (t % SL) * TB);
-      tiles.issue_v(g, t, mine_at + (SL + t % SL) * TB);
-    };
+    auto issue_k = [&](int t) __attribute__((always_inline)) { tiles.issue_k(g, t, mine_at + (t % SL) * TB); };
+    auto issue_v = [&](int t) __attribute__((always_inline)) { tiles.issue_v(g, t, mine_at + (SL + t % SL) * TB); };
     float m_run[MT], l_run[MT];
     f32x4 acc[MT][DB];
 #pragma unroll
@@ -244,8 +244,9 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
     uint64_t there = 0;
 #pragma unroll
     for (int t = 0; t < SL; ++t) {
-      issue(t);
+      issue_k(t);
       there |= (uint64_t)tiles.there(t) << (16 * t);
+      issue_v(t);
     }
     int odd_first = nst, odd_last = -1;  // tiles whose values were not all finite where a row has a hidden key
 #pragma unroll 1
@@ -277,7 +278,10 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
             }
           }
         }
-        vm_wait<2 * NI * (SL - 1)>();
+        lgkm_wait0();  // the slot's keys are read
+        issue_k(t + SL);
+        there = there >> 16 | (uint64_t)tiles.there(t + SL) << (16 * (SL - 1));
+        vm_wait<NI + 2 * NI * (SL - 1)>();
         if (any) {
           i16x4 phi[MT], plo[MT];
 #pragma unroll
@@ -345,9 +349,8 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
             }
           }
         }
-        lgkm_wait0();  // the slot's reads are done
-        issue(t + SL);
-        there = there >> 16 | (uint64_t)tiles.there(t + SL) << (16 * (SL - 1));
+        lgkm_wait0();  // its values are read
+        issue_v(t + SL);
       }
     }
     vm_wait<0>();
