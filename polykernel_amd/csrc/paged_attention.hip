@@ -106,9 +106,9 @@ template <int DP, int DC, bool PAGE16>
 __global__ __launch_bounds__(PC_THREADS, DP == 256 ? 1 : DP == 64 ? 4 : 2) void paged_chunk_kernel(ChunkArgs d) {
   paged_chunk_body<DP, DC, PAGE16>(d);
 }
-template <int DP>
+template <int DP, int DC>
 __global__ __launch_bounds__(PC_THREADS) void paged_chunk_merge_kernel(ChunkArgs d) {
-  paged_chunk_merge_body<DP>(d);
+  paged_chunk_merge_body<DP, DC>(d);
 }
 
 constexpr int PD_LEAST = 1;   // steps of a workgroup
@@ -199,7 +199,7 @@ int run_chunk_as(const ChunkArgs &d, hipStream_t st) {
   else paged_chunk_kernel<DP, DC, false><<<blocks, PC_THREADS, 0, st>>>(d);
   PK_LAUNCH_CHECK("paged_chunk_kernel");
   if (d.splits > 1) {
-    paged_chunk_merge_kernel<DP><<<dim3(d.items, PC_ROWS / PC_MERGE_ROWS), PC_THREADS, 0, st>>>(d);
+    paged_chunk_merge_kernel<DP, DC><<<dim3(d.items, PC_MERGE), PC_THREADS, 0, st>>>(d);
     PK_LAUNCH_CHECK("paged_chunk_merge_kernel");
   }
   return PK_OK;

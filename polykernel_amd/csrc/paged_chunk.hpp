@@ -447,18 +447,16 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
   if (d.splits > 1) {
     // this split's state of the rows
     float *part = d.parts + ((size_t)order * d.splits + it.split) * pc_part_floats(DP);
-    const int r = 32 * wid + col;
-    if (col < wrows) {
 #pragma unroll
-      for (int e = 0; e < DB; ++e)
+    for (int e = 0; e < DB; ++e)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          *reinterpret_cast<f32x4 *>(part + (size_t)r * DP + 32 * e + 8 * j + 4 * h) =
-              f32x4{acc[e][4 * j], acc[e][4 * j + 1], acc[e][4 * j + 2], acc[e][4 * j + 3]};
-      if (h == 0) {
-        part[(size_t)PC_ROWS * DP + 2 * r] = m_run;
-        part[(size_t)PC_ROWS * DP + 2 * r + 1] = l_run;
-      }
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<f32x4 *>(part + (size_t)(((wid * DB + e) * 4 + j) * 64 + lane) * 4) =
+            f32x4{acc[e][4 * j], acc[e][4 * j + 1], acc[e][4 * j + 2], acc[e][4 * j + 3]};
+    if (h == 0) {
+      float *ml = part + (size_t)PC_ROWS * DP + 2 * (32 * wid + col);
+      ml[0] = m_run;
+      ml[1] = l_run;
     }
     return;
   }
@@ -485,32 +483,55 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
   }
 }
 
-// Adds the splits of an item's rows [16 y, + 16) in order, 4 dims of a row per thread.
-constexpr int PC_MERGE_ROWS = 16;
-template <int DP>
+// Adds the splits of an item in order.  A state holds its sums as the lanes have them (four
+// dims of a row; wave, block of 32 dims, run of 8 in it, lane), so that every access is 16
+// bytes a lane in a row; a thread takes one of those and reads AT_ONCE splits before it adds them.
+constexpr int PC_MERGE = 8;  // workgroups of an item
+template <int DP, int DC>
 __device__ __forceinline__ void paged_chunk_merge_body(const ChunkArgs &d) {
+  constexpr int DB = DC / 32, AT_ONCE = 8;
   const AttendArgs &g = d.a;
   Item it;
   int order;
   if (!find_item(d, 1, blockIdx.x, false, it, order)) return;
   const Seq s = it.s;
-  const int G = (int)g.group.d, D = g.cache.dim, cpr = D / 4;
+  const int G = (int)g.group.d, D = g.cache.dim;
   const int row0 = it.tile * PC_ROWS, rows = min(PC_ROWS, s.n * G - row0);
-  const int r0 = blockIdx.y * PC_MERGE_ROWS, n = min(PC_MERGE_ROWS, rows - r0);
   const float c2 = fabsf(g.c2);
   const float *parts = d.parts + (size_t)order * d.splits * pc_part_floats(DP);
-  for (int x = threadIdx.x; x < n * cpr; x += PC_THREADS) {
-    const int r = r0 + x / cpr, dd = 4 * (x % cpr);
+  auto weight = [&](float m, float M) __attribute__((always_inline)) {
+    return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - M) * c2);
+  };
+  for (int x = blockIdx.y * PC_THREADS + threadIdx.x; x < PC_ROWS * DC / 4; x += PC_MERGE * PC_THREADS) {
+    const int lane = x & 63, j = x >> 6 & 3, we = x >> 8, w = we / DB, e = we - w * DB;
+    const int r = 32 * w + (lane & 31), dd = 32 * e + 8 * j + 4 * (lane >> 5);
+    if (r >= rows || dd >= D) continue;
     float M = -INFINITY, L = 0.f;
-    for (int k = 0; k < d.splits; ++k) M = fmaxf(M, parts[k * pc_part_floats(DP) + (size_t)PC_ROWS * DP + 2 * r]);
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < d.splits; ++k) {
-      const float *p = parts + k * pc_part_floats(DP);
-      const float m = p[(size_t)PC_ROWS * DP + 2 * r];
-      if (m == -INFINITY && p[(size_t)PC_ROWS * DP + 2 * r + 1] == 0.f) continue;
-      const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - M) * c2);
-      L += p[(size_t)PC_ROWS * DP + 2 * r + 1] * f;
-      v += *reinterpret_cast<const f32x4 *>(p + (size_t)r * DP + dd) * f;
+    for (int k0 = 0; k0 < d.splits; k0 += AT_ONCE) {
+      float m[AT_ONCE], l[AT_ONCE];
+      f32x4 o[AT_ONCE];
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const float *p = parts + (size_t)min(k0 + i, d.splits - 1) * pc_part_floats(DP);
+        const float2 ml = *reinterpret_cast<const float2 *>(p + (size_t)PC_ROWS * DP + 2 * r);
+        o[i] = *reinterpret_cast<const f32x4 *>(p + 4 * x);
+        m[i] = k0 + i < d.splits ? ml.x : -INFINITY;
+        l[i] = ml.y;
+      }
+      float M2 = M;
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) M2 = fmaxf(M2, m[i]);
+      const float a = weight(M, M2);
+      L *= a;
+      v *= a;
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const float f = weight(m[i], M2);
+        L += l[i] * f;
+        v += o[i] * f;
+      }
+      M = M2;
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
     const int i = (int)g.group.div(row0 + r);
