@@ -247,7 +247,8 @@ typedef struct pk_paged_batch {
                               * are sequence b's; NULL: one token each */
   const int32_t *kv_len;     /* [sequences]: keys of each sequence, the new tokens' among them */
   int sequences, tokens;
-  int max_q;                 /* about the most new tokens of a sequence (only speed depends on it); 0: unknown */
+  int max_q, max_kv;         /* about the most new tokens and the most keys of a sequence (only speed depends on
+                              * them); 0: unknown */
 } pk_paged_batch;
 
 /* Append: token i of the n new ones of sequence b has position p = kv_len[b] -
@@ -276,13 +277,13 @@ PK_API int launch_paged_attention(const pk_tokens *q, const pk_tokens *out, int 
                                   size_t workspace_bytes, void *stream);
 
 /* Test hook: how launch_paged_attention takes a call with 16-byte aligned operands
- * and strides (no device is needed).  dim 0: the general kernel.  step_rows > 0: the
- * step kernel, with that many rows (tokens x query heads of a group) per item and
- * `workgroups`, which cut items between them unless `whole`; splits > 0: the chunk
- * kernel, `items` items at most, each in that many runs of keys.  With both, sequences
- * of up to 64 rows are the step kernel's. */
+ * and strides (no device is needed).  dim 0: the general kernel.  workgroups > 0:
+ * the step kernel, with at most so many, which cut items (16 rows: tokens x query heads
+ * of a group) between them unless `whole`; splits > 0: the chunk kernel, `items` items
+ * (128 rows) at most, each in up to that many runs of keys.  With both, sequences of up
+ * to 16 rows are the step kernel's. */
 typedef struct pk_paged_plan {
-  int dim, step_rows, workgroups, whole, splits, items;
+  int dim, workgroups, whole, splits, items;
 } pk_paged_plan;
 PK_API int pk_paged_attention_plan(int q_heads, const pk_paged_cache *cache, const pk_paged_batch *batch, int window,
                                    pk_paged_plan *out);

@@ -77,14 +77,13 @@ class PagedBatch(C.Structure):
 
     _fields_ = [("page_table", C.c_void_p), ("table_stride", C.c_int64), ("table_width", C.c_int),
                 ("q_start", C.c_void_p), ("kv_len", C.c_void_p), ("sequences", C.c_int), ("tokens", C.c_int),
-                ("max_q", C.c_int)]
+                ("max_q", C.c_int), ("max_kv", C.c_int)]
 
 
 class PagedPlan(C.Structure):
     """struct pk_paged_plan: the kernels of a paged attention call."""
 
-    _fields_ = [("dim", C.c_int), ("step_rows", C.c_int), ("workgroups", C.c_int), ("whole", C.c_int),
-                ("splits", C.c_int), ("items", C.c_int)]
+    _fields_ = [("dim", C.c_int), ("workgroups", C.c_int), ("whole", C.c_int), ("splits", C.c_int), ("items", C.c_int)]
 
 
 ROTARY_SCALINGS = ("none", "linear", "base", "bands", "ramp")

@@ -94,13 +94,13 @@ int run_general(const AttendArgs &g, hipStream_t st) {
 }
 
 // ---- the fast kernels (paged_decode.hpp, paged_chunk.hpp) ------------------------
-template <int DP, int MT, bool PAGE16>
-__global__ __launch_bounds__(PD_THREADS, (DecodeShape<DP, MT>::GROUPS)) void paged_decode_kernel(DecodeArgs d) {
-  paged_decode_body<DP, MT, PAGE16>(d);
+template <int DP, bool PAGE16>
+__global__ __launch_bounds__(PD_THREADS, pd_groups(DP)) void paged_decode_kernel(DecodeArgs d) {
+  paged_decode_body<DP, PAGE16>(d);
 }
-template <int DP, int MT>
+template <int DP>
 __global__ __launch_bounds__(PD_THREADS) void paged_decode_merge_kernel(DecodeArgs d) {
-  paged_decode_merge_body<DP, MT>(d);
+  paged_decode_merge_body<DP>(d);
 }
 template <int DP, int DC, bool PAGE16>
 __global__ __launch_bounds__(PC_THREADS, DP == 256 ? 1 : DP == 64 ? 4 : 2) void paged_chunk_kernel(ChunkArgs d) {
@@ -111,62 +111,85 @@ __global__ __launch_bounds__(PC_THREADS) void paged_chunk_merge_kernel(ChunkArgs
   paged_chunk_merge_body<DP, DC>(d);
 }
 
-constexpr int PD_LEAST = 1;   // steps of a workgroup
-// Workgroups of the step kernel on a CU.
-constexpr int step_groups(int dp, int mt) {
-  return dp == 64    ? mt == 1 ? DecodeShape<64, 1>::GROUPS : mt == 2 ? DecodeShape<64, 2>::GROUPS : DecodeShape<64, 4>::GROUPS
-         : dp == 128 ? mt == 1 ? DecodeShape<128, 1>::GROUPS : mt == 2 ? DecodeShape<128, 2>::GROUPS : DecodeShape<128, 4>::GROUPS
-         : mt == 1   ? DecodeShape<256, 1>::GROUPS
-                     : DecodeShape<256, 2>::GROUPS;
-}
-constexpr int PD_ROWS = 64;   // rows (tokens x heads of a group) of a sequence up to which it is not a chunk
-
 // How a call runs: head dims padded to `dp` (0: by the general kernel); sequences of up to
-// PD_ROWS rows by the decode kernel (mt > 0: 16 mt rows per item, at most `workers`
+// 16 rows (tokens x heads of a group) by the step kernel (workers > 0: at most so many
 // workgroups, items cut between them unless `whole`), sequences of more by the chunk kernel
-// (splits > 0: `items` items at most, each in `splits` runs of keys).  A kernel that runs
-// alone takes all sequences.
+// (splits > 0: `items` items at most, each in up to `splits` runs of keys).  A kernel that
+// runs alone takes all sequences.
+//
+// The step kernel with 32 or 64 rows to an item was slower than the chunk kernel (24
+// sequences of 5 tokens on up to 3000 keys, 8 heads to 32, 50 against 48 us; of 8 tokens 49
+// and 44; 32 of 6, 8 to 56 heads of 64, 45 and 28; 8 of one token on 8000, 1 to 64, 30 and 20).
 struct Choice {
-  int dp = 0, mt = 0, workers = 0, whole = 0, splits = 0, items = 0;
+  int dp = 0, workers = 0, whole = 0, splits = 0, items = 0;
   size_t workspace() const {
     if (!dp) return 0;
-    const size_t few = mt && workers > 1 && !whole ? pd_workspace(dp, mt, workers) : 0;
+    const size_t few = workers > 1 && !whole ? pd_workspace(dp, workers) : 0;
     const size_t many = splits > 1 ? (size_t)items * splits * pc_part_floats(dp) * sizeof(float) : 0;
     return std::max(few, many);
   }
 };
 
+// Runs of keys of the chunk kernel's items: the longest workgroup's steps, a CU's workgroups
+// in so many rounds, against the states that are written and added (66 KB each at D 128).
+// `us`: a step of one workgroup alone on a CU; `shared`: of each more that runs beside it.
+int chunk_splits(int64_t items, int64_t steps, int dp) {
+  const int at_once = dp == 64 ? 4 : dp == 128 ? 2 : 1;
+  const double us = dp == 64 ? 0.8 : dp == 128 ? 1.2 : 2.3, shared = dp == 64 ? 0.6 : dp == 128 ? 0.97 : 2.3;
+  int best = 1;
+  double least = 1e30;
+  for (int s = 1; s <= 32 && (s == 1 || 4 * s <= steps); ++s) {
+    const int64_t groups = items * s, per_cu = (groups + 255) / 256;
+    const double rounds = (double)((per_cu + at_once - 1) / at_once);
+    const double step = std::max(us, shared * std::min<int64_t>(per_cu, at_once));
+    const double time = rounds * (step * ((steps + s - 1) / s) + 3) + (s > 1 ? 3.5 + 0.028 * dp / 128 * groups : 0);
+    if (time < least) {
+      least = time;
+      best = s;
+    }
+  }
+  return best;
+}
+
 Choice choose(int q_heads, const pk_paged_cache &c, const pk_paged_batch &b, int window) {
   Choice r;
   if (c.dim > 256 || c.dim % 8 != 0) return r;
   const int dp = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
-  const int64_t slots = dp == 256 ? 256 : 512;  // chunk workgroups that run at once
-  const int64_t group = q_heads / c.heads;
-  const int64_t steps = (int64_t)b.table_width * c.page_size / PT_STEP + 2;  // of an item, at most
+  const int64_t group = q_heads / c.heads, B = b.sequences;
+  int64_t keys = (int64_t)b.table_width * c.page_size;  // of a sequence, at most
+  if (b.max_kv > 0) keys = std::min<int64_t>(keys, b.max_kv);
+  const int64_t steps = (int64_t)b.table_width * c.page_size / PT_STEP + 2;  // of an item, whatever the hint
   // a hint of fewer tokens than there are on average is none
-  const int64_t most = std::max<int64_t>(b.max_q, ((int64_t)b.tokens + b.sequences - 1) / b.sequences);
+  const int64_t most = std::max<int64_t>(b.max_q, (b.tokens + B - 1) / B);
+  const bool even = (int64_t)b.max_q * B == b.tokens;  // all sequences have the hint's length
   const bool chunks = most * group > PD_ROWS;
-  // Beside chunks the decode kernel takes the others, but not where every sequence is a chunk
-  // (there is one, or all have the hint's length), nor where no token reaches further than the
-  // chunks' own work goes on (mixed batch of 4 prompts of up to 1531 tokens and 20 single ones, D
-  // 64, the last 1024 keys: 54 us and 17 of the decode kernel and its merge, FIGURE with one kernel).
-  const int64_t reach = window > 0 ? std::min<int64_t>((window + PT_KEYS) / PT_STEP + 2, steps) : steps;
-  const bool few = !chunks || !(b.sequences == 1 || (int64_t)b.max_q * b.sequences == b.tokens || reach <= 32);
+  bool few = !chunks;
   if (chunks) {
-    const int64_t items = ((int64_t)b.tokens * group / PC_ROWS + b.sequences) * c.heads;
-    const int64_t splits = std::max<int64_t>(1, std::min<int64_t>({slots / items, steps / 8, 32}));
+    const int64_t items = (b.tokens * group / PC_ROWS + B) * c.heads;
+    // as many as there will be: exactly, or half of the last tiles of sequences
+    const int64_t likely = B == 1 || even ? B * ((b.tokens / B * group + PC_ROWS - 1) / PC_ROWS) * c.heads
+                                          : (b.tokens * group / PC_ROWS + (B + 1) / 2) * c.heads;
+    int64_t reach = keys / PT_STEP + 1;
+    int splits = chunk_splits(likely, reach, dp);
+    if (window > 0) {  // (no more splits than without, which the workspace is for)
+      reach = std::min<int64_t>(reach, (window + PT_KEYS) / PT_STEP + 2);
+      splits = std::min(splits, chunk_splits(likely, reach, dp));
+    }
     if (items * splits > INT32_MAX) return r;
     r.items = (int)items;
-    r.splits = (int)splits;
+    r.splits = splits;
+    // Sequences of few rows beside chunks are the step kernel's, unless all are chunks, or the
+    // few cost the chunk kernel less than another launch and merge: 30 tokens beside 2 chunks of
+    // 500, 8 heads to 32, on up to 1000 keys 61 us with both kernels and 55 with one, 2000 91 and
+    // 86, 4000 135 and 144; 60 beside 2048 on 2000 165 and 214; 8 beside 200 on 3000 60 and 47.
+    few = !(B == 1 || even || B * c.heads * reach <= 8192);
   }
   if (few) {
-    const int64_t rows = chunks ? group : most * group;
-    r.mt = rows <= 16 ? 1 : rows <= 32 || dp == 256 ? 2 : 4;
     // no more workgroups than the tables can have work for
-    const int64_t items = ((int64_t)b.tokens * group / (16 * r.mt) + b.sequences) * c.heads;
-    if (items > INT32_MAX / steps) return r;  // a line of 2^31 steps or more: the general kernel
-    r.whole = steps <= 8;
-    r.workers = (int)std::max<int64_t>(1, std::min<int64_t>(256 * step_groups(dp, r.mt), r.whole ? items : items * steps / PD_LEAST));
+    const int64_t items = (b.tokens * group / PD_ROWS + B) * c.heads;
+    if (items > INT32_MAX / steps) return Choice{};  // a line of 2^31 steps or more: the general kernel
+    r.whole = keys <= 6 * PT_STEP;
+    r.workers = (int)std::max<int64_t>(1, std::min<int64_t>(256 * pd_groups(dp), r.whole ? items : items * steps));
   }
   r.dp = dp;
   return r;
@@ -181,13 +204,13 @@ bool tile_operands(const AttendArgs &g) {
          strides8(c.v_page, c.v_head, c.v_row) && rows(c.k_row) && rows(c.v_row);
 }
 
-template <int DP, int MT>
+template <int DP>
 int run_decode_as(const DecodeArgs &d, hipStream_t st) {
-  if (d.a.cache.page.d % PT_KEYS == 0) paged_decode_kernel<DP, MT, true><<<d.most, PD_THREADS, 0, st>>>(d);
-  else paged_decode_kernel<DP, MT, false><<<d.most, PD_THREADS, 0, st>>>(d);
+  if (d.a.cache.page.d % PT_KEYS == 0) paged_decode_kernel<DP, true><<<d.most, PD_THREADS, 0, st>>>(d);
+  else paged_decode_kernel<DP, false><<<d.most, PD_THREADS, 0, st>>>(d);
   PK_LAUNCH_CHECK("paged_decode_kernel");
   if (d.most > 1 && !d.whole) {
-    paged_decode_merge_kernel<DP, MT><<<d.most - 1, PD_THREADS, 0, st>>>(d);
+    paged_decode_merge_kernel<DP><<<d.most - 1, PD_THREADS, 0, st>>>(d);
     PK_LAUNCH_CHECK("paged_decode_merge_kernel");
   }
   return PK_OK;
@@ -206,16 +229,12 @@ int run_chunk_as(const ChunkArgs &d, hipStream_t st) {
 }
 template <int DP>
 int run_as(const AttendArgs &g, const Choice &c, float *workspace, hipStream_t st) {
-  if (c.mt) {
-    const DecodeArgs d{g, workspace, c.whole ? 1 : PD_LEAST, c.workers, c.splits ? PD_ROWS + 1 : INT32_MAX, c.whole};
-    int rc = PK_OK;
-    if (c.mt == 1) rc = run_decode_as<DP, 1>(d, st);
-    else if (c.mt == 2 || DP == 256) rc = run_decode_as<DP, 2>(d, st);
-    else rc = run_decode_as<DP, DP == 256 ? 2 : 4>(d, st);
-    if (rc) return rc;
+  if (c.workers) {
+    const DecodeArgs d{g, workspace, c.workers, c.splits ? PD_ROWS + 1 : INT32_MAX, c.whole};
+    if (int rc = run_decode_as<DP>(d, st)) return rc;
   }
   if (c.splits) {
-    const ChunkArgs d{g, workspace, c.items, c.splits, c.mt ? PD_ROWS : 0};
+    const ChunkArgs d{g, workspace, c.items, c.splits, c.workers ? PD_ROWS : 0};
     // three quarters of the dims are products enough for head dims up to there
     if constexpr (DP > 64)
       if (g.cache.dim <= DP / 4 * 3) return run_chunk_as<DP, DP / 4 * 3>(d, st);
@@ -242,7 +261,7 @@ int pk_paged_attention_plan(int q_heads, const pk_paged_cache *cache, const pk_p
   if (int rc = check_batch(who, batch, cache, &b)) return rc;
   PK_CHECK_ARG(out && q_heads > 0 && q_heads % cache->heads == 0 && window >= 0 && batch->sequences > 0, "%s: invalid argument", who);
   const Choice r = choose(q_heads, *cache, *batch, window >= b.capacity ? 0 : window);
-  *out = pk_paged_plan{r.dp, 16 * r.mt, r.workers, r.whole, r.splits, r.items};
+  *out = pk_paged_plan{r.dp, r.workers, r.whole, r.splits, r.items};
   return PK_OK;
 }
 

@@ -33,6 +33,9 @@ struct ChunkArgs {
 };
 constexpr size_t pc_part_floats(int DP) { return (size_t)PC_ROWS * (DP + 2); }
 
+// The runs of keys that an item of so many steps is cut into: at least four steps each.
+__device__ __forceinline__ int splits_of(const ChunkArgs &d, int steps) { return min(d.splits, max(1, steps / 4)); }
+
 // An item: 128 rows of one sequence and key head.
 struct Item {
   Seq s;
@@ -90,6 +93,15 @@ __device__ __forceinline__ bool find_item(const ChunkArgs &d, int splits, int i,
   return order < d.items;
 }
 
+// The item's first key (of a tile) and its steps.
+__device__ __forceinline__ int item_steps(const AttendArgs &g, const Item &it, int rows, int &klo, int &hi_all, int &lo_all, int &hi) {
+  int lo;
+  key_range(g, it.s, (int)g.group.div(it.tile * PC_ROWS), lo, hi_all);
+  key_range(g, it.s, (int)g.group.div(it.tile * PC_ROWS + rows - 1), lo_all, hi);
+  klo = lo & ~(PT_KEYS - 1);
+  return max(1, (hi - klo + PC_STEP - 1) / PC_STEP);
+}
+
 // A barrier that waits for this wave's LDS accesses and no loads in flight.
 __device__ __forceinline__ void lds_barrier() {
   lgkm_wait0();
@@ -132,12 +144,10 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
   const int wrow = row0 + 32 * wid, wrows = min(32, all_rows - wrow);  // this wave's (may be none)
 
   // the item's keys, and those that all of this wave's rows see
-  int lo_first, hi_last, t0, t1;
-  key_range(g, s, (int)g.group.div(row0), lo_first, t0);
-  key_range(g, s, (int)g.group.div(row0 + rows - 1), t1, hi_last);
-  const int klo = lo_first & ~(PT_KEYS - 1);
-  const int steps = max(1, (hi_last - klo + PC_STEP - 1) / PC_STEP);
-  const int s0 = (int)((int64_t)steps * it.split / d.splits), nst = (int)((int64_t)steps * (it.split + 1) / d.splits) - s0;
+  int klo, hi_last, t0, t1;
+  const int steps = item_steps(g, it, rows, klo, t0, t1, hi_last), splits = splits_of(d, steps);
+  if (it.split >= splits) return;
+  const int s0 = (int)((int64_t)steps * it.split / splits), nst = (int)((int64_t)steps * (it.split + 1) / splits) - s0;
   const int kfirst = klo + s0 * PC_STEP;
   Tiles tiles(g);
   tiles.begin(g, it.b, it.hk, kfirst + wid * PT_KEYS, nst, hi_last);
@@ -444,7 +454,7 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
         }
   }
 
-  if (d.splits > 1) {
+  if (splits > 1) {
     // this split's state of the rows
     float *part = d.parts + ((size_t)order * d.splits + it.split) * pc_part_floats(DP);
 #pragma unroll
@@ -498,6 +508,9 @@ __device__ __forceinline__ void paged_chunk_merge_body(const ChunkArgs &d) {
   const int G = (int)g.group.d, D = g.cache.dim;
   const int row0 = it.tile * PC_ROWS, rows = min(PC_ROWS, s.n * G - row0);
   const float c2 = fabsf(g.c2);
+  int t0, t1, t2, t3;
+  const int splits = splits_of(d, item_steps(g, it, rows, t0, t1, t2, t3));
+  if (splits == 1) return;  // the kernel wrote the rows
   const float *parts = d.parts + (size_t)order * d.splits * pc_part_floats(DP);
   auto weight = [&](float m, float M) __attribute__((always_inline)) {
     return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - M) * c2);
@@ -508,15 +521,15 @@ __device__ __forceinline__ void paged_chunk_merge_body(const ChunkArgs &d) {
     if (r >= rows || dd >= D) continue;
     float M = -INFINITY, L = 0.f;
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int k0 = 0; k0 < d.splits; k0 += AT_ONCE) {
+    for (int k0 = 0; k0 < splits; k0 += AT_ONCE) {
       float m[AT_ONCE], l[AT_ONCE];
       f32x4 o[AT_ONCE];
 #pragma unroll
       for (int i = 0; i < AT_ONCE; ++i) {
-        const float *p = parts + (size_t)min(k0 + i, d.splits - 1) * pc_part_floats(DP);
+        const float *p = parts + (size_t)min(k0 + i, splits - 1) * pc_part_floats(DP);
         const float2 ml = *reinterpret_cast<const float2 *>(p + (size_t)PC_ROWS * DP + 2 * r);
         o[i] = *reinterpret_cast<const f32x4 *>(p + 4 * x);
-        m[i] = k0 + i < d.splits ? ml.x : -INFINITY;
+        m[i] = k0 + i < splits ? ml.x : -INFINITY;
         l[i] = ml.y;
       }
       float M2 = M;

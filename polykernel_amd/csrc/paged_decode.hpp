@@ -3,8 +3,8 @@
 // What bounds it: keys and values are read once for the G query heads that share
 // them (and the few new tokens), so the time is that of streaming them from HBM.
 //
-// A row is a (token, query head of the group) pair; 16 MT rows of one sequence and
-// key head are one item.  Both products run on the matrix units, transposed: S^T =
+// A row is a (token, query head of the group) pair; 16 rows of one sequence and key
+// head are one item.  Both products run on the matrix units, transposed: S^T =
 // K Q^T (16x16x32, keys x rows) leaves each lane one row and 4 keys of 16, which is
 // the B operand of O^T = V^T P^T (16x16x16), its A operand read from V's rows in LDS
 // by transposing reads.  So P stays in registers; P is split into two bf16 halves
@@ -31,12 +31,12 @@
 namespace pk {
 namespace paged {
 
-constexpr int PD_WAVES = 4, PD_THREADS = PD_WAVES * 64, PD_TILE = PT_KEYS, PD_STEP = PT_STEP;
+constexpr int PD_WAVES = 4, PD_THREADS = PD_WAVES * 64, PD_TILE = PT_KEYS, PD_STEP = PT_STEP, PD_ROWS = 16;
 
-// Bytes of one workgroup's partial state: 16 MT rows of DP sums, and (maximum, sum).
-constexpr size_t pd_part_floats(int DP, int MT) { return (size_t)16 * MT * (DP + 2); }
-constexpr size_t pd_workspace(int DP, int MT, int workers) {
-  return workers * (2 * pd_part_floats(DP, MT) * sizeof(float) + 32);
+// Bytes of one workgroup's partial state: 16 rows of DP sums, and (maximum, sum).
+constexpr size_t pd_part_floats(int DP) { return (size_t)PD_ROWS * (DP + 2); }
+constexpr size_t pd_workspace(int DP, int workers) {
+  return workers * (2 * pd_part_floats(DP) * sizeof(float) + 32);
 }
 
 // Where a workgroup's part begins inside an item: the item's workgroups and rows, for the merge.
@@ -47,7 +47,6 @@ struct Cut {
 struct DecodeArgs {
   AttendArgs a;
   float *parts;  // two partial states per workgroup, then a Cut each
-  int least;     // steps per workgroup, where there are enough for all
   int most;      // workgroups
   int below;     // rows of a sequence from which on another kernel takes it
   int whole;     // items are not cut: a step of the line is an item
@@ -61,7 +60,6 @@ struct Line {
   int unit;               // places of the line that an item takes
   int units;
 };
-template <int ROWS>
 __device__ __forceinline__ Line line_of(const DecodeArgs &d, const Seq &s) {
   const AttendArgs &g = d.a;
   Line l{0, 0, 0, 1, 0};
@@ -70,7 +68,7 @@ __device__ __forceinline__ Line line_of(const DecodeArgs &d, const Seq &s) {
   key_range(g, s, 0, lo, hi);
   key_range(g, s, s.n - 1, lo2, hi2);
   l.klo = lo & ~(PD_TILE - 1);
-  l.tiles = (int)(((int64_t)s.n * (int)g.group.d + ROWS - 1) / ROWS);
+  l.tiles = (int)(((int64_t)s.n * (int)g.group.d + PD_ROWS - 1) / PD_ROWS);
   l.steps = max(1, (hi2 - l.klo + PD_STEP - 1) / PD_STEP);
   l.unit = d.whole ? 1 : l.steps;
   l.units = l.tiles * g.cache.heads * l.unit;
@@ -97,23 +95,28 @@ __device__ __forceinline__ Seq sequence_at(const Batch &g, const Place &p, int b
 }
 // Where workgroup w's part begins, found by every wave for itself: lane l adds up the
 // sequences [l, l + 1) * ceil(B / 64), and a scan over the lanes gives each its offset.
-template <int ROWS>
 __device__ __forceinline__ bool find_place(const DecodeArgs &d, int w, Place &p) {
   const AttendArgs &g = d.a;
   const int lane = threadIdx.x & 63, B = g.batch.sequences;
   const int per = (B + 63) / 64;
-  int mine = 0;
+  int mine = 0, longest = 0;
   p.mine = Seq{0, 0, 0};
   for (int i = 0; i < per; ++i) {
     const int b = lane * per + i;
     if (b < B) {
       p.mine = sequence(g.batch, b);
-      mine += line_of<ROWS>(d, p.mine).units;
+      const Line l = line_of(d, p.mine);
+      mine += l.units;
+      longest = max(longest, l.unit);
     }
   }
   const int incl = wave_scan(mine);
   p.total = __builtin_amdgcn_readlane(incl, 63);
-  p.workers = min(d.most, max(1, p.total / d.least));
+  // a step per workgroup, where there are so few; two where one item has over 256, whose parts
+  // would take longer to add than the steps (1 head of 30000 keys 14.1 against 12.4 us; of 4000
+  // 10.6 against 12.0)
+  const bool two = !d.whole && __any(longest > 256);
+  p.workers = min(d.most, max(1, two ? p.total / 2 : p.total));
   if (w >= p.workers || p.total <= 0) return false;
   p.each = p.total / p.workers;
   p.more = p.total - p.each * p.workers;
@@ -125,7 +128,7 @@ __device__ __forceinline__ bool find_place(const DecodeArgs &d, int w, Place &p)
   int at = __builtin_amdgcn_readlane(incl - mine, l), b = l * per;
   for (;; ++b) {
     if (b >= B) return false;
-    const int n = line_of<ROWS>(d, sequence_at(g.batch, p, b)).units;
+    const int n = line_of(d, sequence_at(g.batch, p, b)).units;
     if (p.first < at + n) {
       p.b = uniform(b);
       p.in_seq = uniform(p.first - at);
@@ -135,25 +138,21 @@ __device__ __forceinline__ bool find_place(const DecodeArgs &d, int w, Place &p)
   }
 }
 
-template <int DP, int MT>
+template <int DP>
 struct DecodeShape {
   static constexpr int NI = TileLoader<DP, true, true>::NI, TB = TileLoader<DP, true, true>::BYTES;
-  static constexpr int SL = DP == 64 ? 2 : 1;  // tiles of a ring
-  static constexpr int PS = DP + 4;            // row stride of a state in LDS, floats
-  static constexpr int STATE = 16 * PS * 4;    // a wave's 16 rows of sums, then its (maximum, sum) of all rows
-  static constexpr int WAVE = 2 * SL * TB > STATE + 128 * MT ? 2 * SL * TB : STATE + 128 * MT;  // its rings, later its state
-  static constexpr int GROUPS = MT == 1 ? (DP == 256 ? 2 : 4) : DP == 256 ? 1 : MT == 2 ? 3 : 2;  // workgroups on a CU
+  static constexpr int SL = DP == 64 ? 2 : 1;      // tiles of a ring
+  static constexpr int PS = DP + 4;                // row stride of a state in LDS, floats
+  static constexpr int STATE = PD_ROWS * PS * 4;   // a wave's sums, then (maximum, sum) of its rows
+  static constexpr int WAVE = 2 * SL * TB > STATE + 8 * PD_ROWS ? 2 * SL * TB : STATE + 8 * PD_ROWS;  // its rings, later its state
 };
+constexpr int pd_groups(int DP) { return DP == 256 ? 2 : 4; }  // workgroups on a CU
 
-template <int DP, int MT, bool PAGE16>
+template <int DP, bool PAGE16>
 __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
-  using S = DecodeShape<DP, MT>;
-  constexpr int CH = DP / 8, NI = S::NI, TB = S::TB, SL = S::SL, PS = S::PS;
-  constexpr int ROWS = 16 * MT, KS = DP / 32, DB = DP / 16;
-  // many query fragments are read from LDS at each tile (the waves share them), few stay in registers
-  constexpr bool QLDS = MT * KS > 8;
-  __shared__ __attribute__((aligned(1024))) uint8_t ring[PD_WAVES * S::WAVE + (QLDS ? ROWS * DP * 2 : 0)];
-  uint8_t *const qs = ring + PD_WAVES * S::WAVE;
+  using S = DecodeShape<DP>;
+  constexpr int CH = DP / 8, NI = S::NI, TB = S::TB, SL = S::SL, PS = S::PS, KS = DP / 32, DB = DP / 16;
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[PD_WAVES * S::WAVE];
   auto ml = [&](int w, int r) __attribute__((always_inline)) {
     return reinterpret_cast<float *>(ring + w * S::WAVE + S::STATE) + 2 * r;
   };
@@ -166,10 +165,10 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
   const uint32_t mine_at = lds_number(ring) + wid * S::WAVE;
 
   auto cut = [&](int w) __attribute__((always_inline)) {
-    return reinterpret_cast<Cut *>(d.parts + (size_t)(2 * d.most) * pd_part_floats(DP, MT)) + w;
+    return reinterpret_cast<Cut *>(d.parts + (size_t)(2 * d.most) * pd_part_floats(DP)) + w;
   };
   Place at;
-  if (!find_place<ROWS>(d, blockIdx.x, at)) {
+  if (!find_place(d, blockIdx.x, at)) {
     if (tid == 0 && d.most > 1 && !d.whole) cut(blockIdx.x)->first = -1;
     return;
   }
@@ -179,7 +178,7 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
   bool first_segment = true;
   while (u < at.last && b < g.batch.sequences) {
     const Seq s = sequence_at(g.batch, at, b);
-    const Line ln = line_of<ROWS>(d, s);
+    const Line ln = line_of(d, s);
     if (in_seq >= ln.units) {
       in_seq = 0;
       ++b;
@@ -188,7 +187,7 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
     const int item = uniform(in_seq / ln.unit), st0 = uniform(in_seq - item * ln.unit);
     const int took = uniform(min(ln.unit - st0, at.last - u)), nst = d.whole ? ln.steps : took;
     const int hk = uniform(item / ln.tiles), tile = item - hk * ln.tiles;
-    const int row0 = tile * ROWS, rows = min(ROWS, s.n * (int)g.group.d - row0);
+    const int row0 = tile * PD_ROWS, rows = min(PD_ROWS, s.n * (int)g.group.d - row0);
 
     // the keys that all rows of the tile see, and those that any does
     int lo_any, hi_all, lo_all, hi_any;
@@ -199,47 +198,29 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
     const int key0 = ln.klo + st0 * PD_STEP + wid * PD_TILE;
     tiles.begin(g, b, hk, key0, nst, hi_any);  // before the queries' loads: loads return in order
 
-    int lo[MT], hi[MT];
-    bf16x8 qf[QLDS ? 1 : MT][KS];
-    if constexpr (QLDS) {
-      for (int x = tid; x < ROWS * CH; x += PD_THREADS) {
-        const int r = x / CH, c = x % CH;
-        const int i = (int)g.group.div(row0 + min(r, rows - 1)), h = hk * (int)g.group.d + row0 + min(r, rows - 1) - i * (int)g.group.d;
-        att::u32x4 v = {0, 0, 0, 0};
-        if (8 * c < D) v = *reinterpret_cast<const att::u32x4 *>(g.q.data + (int64_t)(s.q0 + i) * g.q.token + h * g.q.head + 8 * c);
-        if (g.c2 < 0.f) v ^= 0x80008000u;
-        *reinterpret_cast<att::u32x4 *>(qs + r * DP * 2 + 16 * att::swz_k<CH>(c, r)) = v;
-      }
-      __syncthreads();
-    }
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int r = min(row0 + 16 * m + col, row0 + rows - 1);
+    int lo, hi;
+    bf16x8 qf[KS];
+    {
+      const int r = min(row0 + col, row0 + rows - 1);
       const int i = (int)g.group.div(r), h = hk * (int)g.group.d + r - i * (int)g.group.d;
-      key_range(g, s, i, lo[m], hi[m]);
-      if constexpr (QLDS) continue;
+      key_range(g, s, i, lo, hi);
       const uint16_t *qp = g.q.data + (int64_t)(s.q0 + i) * g.q.token + h * g.q.head + 8 * grp;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         att::u32x4 v = {0, 0, 0, 0};
         if (32 * k + 8 * grp < D) v = *reinterpret_cast<const att::u32x4 *>(qp + 32 * k);
         if (g.c2 < 0.f) v ^= 0x80008000u;
-        qf[QLDS ? 0 : m][k] = __builtin_bit_cast(bf16x8, v);
+        qf[k] = __builtin_bit_cast(bf16x8, v);
       }
     }
     const float c2 = fabsf(g.c2);
 
     auto issue_k = [&](int t) __attribute__((always_inline)) { tiles.issue_k(g, t, mine_at + (t % SL) * TB); };
     auto issue_v = [&](int t) __attribute__((always_inline)) { tiles.issue_v(g, t, mine_at + (SL + t % SL) * TB); };
-    float m_run[MT], l_run[MT];
-    f32x4 acc[MT][DB];
+    float m_run = -INFINITY, l_run = 0.f;
+    f32x4 acc[DB];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      m_run[m] = -INFINITY;
-      l_run[m] = 0.f;
-#pragma unroll
-      for (int e = 0; e < DB; ++e) acc[m][e] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+    for (int e = 0; e < DB; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
     // which keys of the next SL tiles are there, 16 bits each: looked up when a tile is issued
     uint64_t there = 0;
 #pragma unroll
@@ -251,170 +232,141 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
     int odd_first = nst, odd_last = -1;  // tiles whose values were not all finite where a row has a hidden key
 #pragma unroll 1
     for (int t = 0; t < nst; ++t) {
-      {
-        const int o = t % SL;
-        const int key = key0 + t * PD_STEP;
-        uint8_t *ks = mine + o * TB, *vs = mine + (SL + o) * TB;
-        const uint32_t here = (uint32_t)there & 0xFFFFu;
-        const bool any = key < hi_any && here != 0;
-        const bool masked = key < lo_all || key + PD_TILE > hi_all || here != 0xFFFFu;
-        f32x4 sc[MT];
-        vm_wait<NI + 2 * NI * (SL - 1)>();
-        if (any) {
-          bf16x8 kf[KS];
+      const int key = key0 + t * PD_STEP;
+      const uint8_t *ks = mine + (t % SL) * TB;
+      uint8_t *vs = mine + (SL + t % SL) * TB;
+      const uint32_t here = (uint32_t)there & 0xFFFFu;
+      const bool any = key < hi_any && here != 0;
+      const bool masked = key < lo_all || key + PD_TILE > hi_all || here != 0xFFFFu;
+      f32x4 sc = {0.f, 0.f, 0.f, 0.f};
+      vm_wait<NI + 2 * NI * (SL - 1)>();
+      if (any) {
 #pragma unroll
-          for (int k = 0; k < KS; ++k)
-            kf[k] = __builtin_bit_cast(
-                bf16x8, *reinterpret_cast<const att::u32x4 *>(ks + col * DP * 2 + 16 * att::swz_k<CH>(4 * k + grp, col)));
+        for (int k = 0; k < KS; ++k) {
+          const att::u32x4 kv = *reinterpret_cast<const att::u32x4 *>(ks + col * DP * 2 + 16 * att::swz_k<CH>(4 * k + grp, col));
+          sc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kv), qf[k], sc, 0, 0, 0);
+        }
+      }
+      lgkm_wait0();  // the slot's keys are read
+      issue_k(t + SL);
+      there = there >> 16 | (uint64_t)tiles.there(t + SL) << (16 * (SL - 1));
+      vm_wait<NI + 2 * NI * (SL - 1)>();
+      if (any) {
+        if (masked) {
 #pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            sc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
-              if constexpr (QLDS)
-                qf[0][k] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const att::u32x4 *>(
-                                                          qs + (16 * m + col) * DP * 2 + 16 * att::swz_k<CH>(4 * k + grp, col)));
-              sc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[k], qf[QLDS ? 0 : m][k], sc[m], 0, 0, 0);
-            }
+          for (int i = 0; i < 4; ++i) {
+            const int kk = 4 * grp + i;
+            if (key + kk < lo || key + kk >= hi || !(here >> kk & 1)) sc[i] = -INFINITY;
           }
         }
-        lgkm_wait0();  // the slot's keys are read
-        issue_k(t + SL);
-        there = there >> 16 | (uint64_t)tiles.there(t + SL) << (16 * (SL - 1));
-        vm_wait<NI + 2 * NI * (SL - 1)>();
-        if (any) {
-          i16x4 phi[MT], plo[MT];
+        float top = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+        top = xor32_max(top);
+        float a0, a1;
+        att::xor16_pair(top, top, a0, a1);
+        top = fmaxf(a0, a1);
+        // the maximum in the exponent follows once it is 2^8 behind: sums of p v / p do not depend on it
+        if (__any((top - m_run) * c2 > 8.f)) {
+          const float m_new = fmaxf(m_run, top);
+          const float alpha = m_run == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run - m_new) * c2);
+          m_run = m_new;
+          l_run *= alpha;
 #pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            if (masked) {
+          for (int e = 0; e < DB; ++e) acc[e] *= alpha;
+        }
+        const float mc = m_run == -INFINITY ? 0.f : m_run * c2;
+        float p[4];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int kk = 4 * grp + i;
-                if (key + kk < lo[m] || key + kk >= hi[m] || !(here >> kk & 1)) sc[m][i] = -INFINITY;
-              }
-            }
-            float top = fmaxf(fmaxf(sc[m][0], sc[m][1]), fmaxf(sc[m][2], sc[m][3]));
-            top = xor32_max(top);
-            float a0, a1;
-            att::xor16_pair(top, top, a0, a1);
-            top = fmaxf(a0, a1);
-            // the maximum in the exponent follows once it is 2^8 behind: sums of p v / p do not depend on it
-            if (__any((top - m_run[m]) * c2 > 8.f)) {
-              const float m_new = fmaxf(m_run[m], top);
-              const float alpha = m_run[m] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m_run[m] - m_new) * c2);
-              m_run[m] = m_new;
-              l_run[m] *= alpha;
+        for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], c2, -mc));
+        l_run += (p[0] + p[1]) + (p[2] + p[3]);
+        const uint32_t h0 = pack_bf(p[0], p[1]), h1 = pack_bf(p[2], p[3]);
+        const i16x4 phi = __builtin_bit_cast(i16x4, (att::u32x2{h0, h1}));
+        const i16x4 plo = __builtin_bit_cast(i16x4, (att::u32x2{pack_bf(p[0] - lo_bf(h0), p[1] - hi_bf(h0)),
+                                                                pack_bf(p[2] - lo_bf(h1), p[3] - hi_bf(h1))}));
+        if (masked) {
+          pk_u16x2 most = {0, 0};
+#pragma unroll 1
+          for (int i = 0; i < NI; ++i) {
+            const att::u32x4 w = *reinterpret_cast<const att::u32x4 *>(vs + i * 1024 + 16 * lane);
 #pragma unroll
-              for (int e = 0; e < DB; ++e) acc[m][e] *= alpha;
-            }
-            const float mc = m_run[m] == -INFINITY ? 0.f : m_run[m] * c2;
-            float p[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(fmaf(sc[m][i], c2, -mc));
-            l_run[m] += (p[0] + p[1]) + (p[2] + p[3]);
-            const uint32_t h0 = pack_bf(p[0], p[1]), h1 = pack_bf(p[2], p[3]);
-            phi[m] = __builtin_bit_cast(i16x4, (att::u32x2{h0, h1}));
-            plo[m] = __builtin_bit_cast(i16x4, (att::u32x2{pack_bf(p[0] - lo_bf(h0), p[1] - hi_bf(h0)),
-                                                           pack_bf(p[2] - lo_bf(h1), p[3] - hi_bf(h1))}));
+            for (int e = 0; e < 4; ++e) most = exponents(most, w[e]);
           }
-          if (masked) {
-            pk_u16x2 most = {0, 0};
+          if (__any(not_finite(most))) {
+            odd_first = min(odd_first, t);
+            odd_last = t;
 #pragma unroll 1
             for (int i = 0; i < NI; ++i) {
-              const att::u32x4 w = *reinterpret_cast<const att::u32x4 *>(vs + i * 1024 + 16 * lane);
+              att::u32x4 *at = reinterpret_cast<att::u32x4 *>(vs + i * 1024 + 16 * lane), w = *at;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) most = exponents(most, w[e]);
-            }
-            if (__any(not_finite(most))) {
-              odd_first = min(odd_first, t);
-              odd_last = t;
-#pragma unroll 1
-              for (int i = 0; i < NI; ++i) {
-                att::u32x4 *at = reinterpret_cast<att::u32x4 *>(vs + i * 1024 + 16 * lane), w = *at;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = finite(w[e]);
-                *at = w;
-              }
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < DB; ++e) {
-            const int key_r = 4 * grp + (col >> 2), c = 2 * e + (col & 3) / 2;
-            const i16x4 vf = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (att::lds_i16x4 *)(vs + key_r * DP * 2 + 16 * (c ^ att::swz_v<DP>(key_r)) + 8 * (col & 1)));
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-              acc[m][e] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vf, phi[m], acc[m][e], 0, 0, 0);
-              acc[m][e] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vf, plo[m], acc[m][e], 0, 0, 0);
+              for (int e = 0; e < 4; ++e) w[e] = finite(w[e]);
+              *at = w;
             }
           }
         }
-        lgkm_wait0();  // its values are read
-        issue_v(t + SL);
+#pragma unroll
+        for (int e = 0; e < DB; ++e) {
+          const int key_r = 4 * grp + (col >> 2), c = 2 * e + (col & 3) / 2;
+          const i16x4 vf = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (att::lds_i16x4 *)(vs + key_r * DP * 2 + 16 * (c ^ att::swz_v<DP>(key_r)) + 8 * (col & 1)));
+          acc[e] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vf, phi, acc[e], 0, 0, 0);
+          acc[e] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vf, plo, acc[e], 0, 0, 0);
+        }
       }
+      lgkm_wait0();  // its values are read
+      issue_v(t + SL);
     }
     vm_wait<0>();
     for (int t = odd_first; t <= odd_last; ++t)
       for (int k = key0 + t * PD_STEP; k < min(hi_any, key0 + t * PD_STEP + PD_TILE); ++k) {
         const uint16_t *vr = value_row(g, b, hk, k);
-        if (!vr) continue;
+        if (!vr || k < lo || k >= hi) continue;
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-          if (k >= lo[m] && k < hi[m])
-#pragma unroll
-            for (int e = 0; e < DB; ++e)
-              if (16 * e + 4 * grp < D) add_not_finite(vr + 16 * e + 4 * grp, acc[m][e]);
+        for (int e = 0; e < DB; ++e)
+          if (16 * e + 4 * grp < D) add_not_finite(vr + 16 * e + 4 * grp, acc[e]);
       }
 
     // ---- the waves' states, added in wave order
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
+    {
       float x0, x1;
-      l_run[m] = xor32_sum(l_run[m]);
-      att::xor16_pair(l_run[m], l_run[m], x0, x1);
-      l_run[m] = x0 + x1;
+      l_run = xor32_sum(l_run);
+      att::xor16_pair(l_run, l_run, x0, x1);
       if (grp == 0) {
-        ml(wid, 16 * m + col)[0] = m_run[m];
-        ml(wid, 16 * m + col)[1] = l_run[m];
+        ml(wid, col)[0] = m_run;
+        ml(wid, col)[1] = x0 + x1;
       }
-    }
-    const bool whole = nst == ln.steps;
-    float *part = d.parts + (size_t)(2 * blockIdx.x + (first_segment ? 0 : 1)) * pd_part_floats(DP, MT);
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
       float *so = reinterpret_cast<float *>(mine);
 #pragma unroll
-      for (int e = 0; e < DB; ++e) *reinterpret_cast<f32x4 *>(so + col * PS + 16 * e + 4 * grp) = acc[m][e];
-      __syncthreads();
-      for (int x = tid; x < 16 * (DP / 4); x += PD_THREADS) {
-        const int rr = x / (DP / 4), dd = 4 * (x % (DP / 4)), r = 16 * m + rr;
-        if (r >= rows) continue;
-        float M = -INFINITY, L = 0.f;
+      for (int e = 0; e < DB; ++e) *reinterpret_cast<f32x4 *>(so + col * PS + 16 * e + 4 * grp) = acc[e];
+    }
+    __syncthreads();
+    const bool whole = nst == ln.steps;
+    float *part = d.parts + (size_t)(2 * blockIdx.x + (first_segment ? 0 : 1)) * pd_part_floats(DP);
+    for (int x = tid; x < rows * (DP / 4); x += PD_THREADS) {
+      const int r = x / (DP / 4), dd = 4 * (x % (DP / 4));
+      if (dd >= D) continue;
+      float M = -INFINITY, L = 0.f;
 #pragma unroll
-        for (int w = 0; w < PD_WAVES; ++w) M = fmaxf(M, ml(w, r)[0]);
-        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+      for (int w = 0; w < PD_WAVES; ++w) M = fmaxf(M, ml(w, r)[0]);
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < PD_WAVES; ++w) {
-          const float mw = ml(w, r)[0], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw - M) * c2);
-          L += ml(w, r)[1] * f;
-          v += *reinterpret_cast<const f32x4 *>(ring + w * S::WAVE + (rr * PS + dd) * 4) * f;
-        }
-        if (whole) {
-          if (dd >= D) continue;
-          const float inv = L == 0.f ? 0.f : 1.f / L;
-          const int i = (int)g.group.div(row0 + r), h = hk * (int)g.group.d + row0 + r - i * (int)g.group.d;
-          *reinterpret_cast<att::u32x2 *>(g.out.data + (int64_t)(s.q0 + i) * g.out.token + h * g.out.head + dd) =
-              att::u32x2{pack_bf(v[0] * inv, v[1] * inv), pack_bf(v[2] * inv, v[3] * inv)};
-        } else {
-          *reinterpret_cast<f32x4 *>(part + (size_t)r * DP + dd) = v;
-          if (dd == 0) {
-            part[(size_t)ROWS * DP + 2 * r] = M;
-            part[(size_t)ROWS * DP + 2 * r + 1] = L;
-          }
+      for (int w = 0; w < PD_WAVES; ++w) {
+        const float mw = ml(w, r)[0], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((mw - M) * c2);
+        L += ml(w, r)[1] * f;
+        v += *reinterpret_cast<const f32x4 *>(ring + w * S::WAVE + (r * PS + dd) * 4) * f;
+      }
+      if (whole) {
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const int i = (int)g.group.div(row0 + r), h = hk * (int)g.group.d + row0 + r - i * (int)g.group.d;
+        *reinterpret_cast<att::u32x2 *>(g.out.data + (int64_t)(s.q0 + i) * g.out.token + h * g.out.head + dd) =
+            att::u32x2{pack_bf(v[0] * inv, v[1] * inv), pack_bf(v[2] * inv, v[3] * inv)};
+      } else {
+        *reinterpret_cast<f32x4 *>(part + (size_t)r * DP + dd) = v;
+        if (dd == 0) {
+          part[(size_t)PD_ROWS * DP + 2 * r] = M;
+          part[(size_t)PD_ROWS * DP + 2 * r + 1] = L;
         }
       }
-      __syncthreads();
     }
+    __syncthreads();
     if (first_segment && tid == 0 && d.most > 1 && !d.whole) {
       Cut c{-1, 0, 0, s.q0, hk, row0, rows, 0};
       if (st0 > 0) {
@@ -435,13 +387,13 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
 // of this launch numbered first + 1 to last share its outputs, 4 dims of a row (a chunk) at a
 // time.  A thread reads AT_ONCE parts of a chunk before it adds them; more parts have more
 // threads (a power of two up to 32), whose sums meet in LDS.
-template <int DP, int MT>
+template <int DP>
 __device__ __forceinline__ void paged_decode_merge_body(const DecodeArgs &d) {
-  constexpr int ROWS = 16 * MT, AT_ONCE = 4;
+  constexpr int AT_ONCE = 4;
   __shared__ float sum[PD_THREADS][6];
   const AttendArgs &g = d.a;
   const int w = blockIdx.x + 1;
-  const size_t stride = pd_part_floats(DP, MT);
+  const size_t stride = pd_part_floats(DP);
   const Cut cut = reinterpret_cast<const Cut *>(d.parts + (size_t)(2 * d.most) * stride)[w];
   const int w0 = cut.first, w1 = cut.last, rows = cut.rows, D = g.cache.dim;
   if (w0 < 0) return;
@@ -465,7 +417,7 @@ __device__ __forceinline__ void paged_decode_merge_body(const DecodeArgs &d) {
       for (int i = 0; i < AT_ONCE; ++i) {
         const int k = min(k0 + i * groups, w1);
         const float *p = k == w0 ? p0 : d.parts + (size_t)(2 * k) * stride;
-        const float2 ml = *reinterpret_cast<const float2 *>(p + (size_t)ROWS * DP + 2 * r);
+        const float2 ml = *reinterpret_cast<const float2 *>(p + (size_t)PD_ROWS * DP + 2 * r);
         o[i] = *reinterpret_cast<const f32x4 *>(p + (size_t)r * DP + dd);
         m[i] = k0 + i * groups <= w1 ? ml.x : -INFINITY;
         l[i] = ml.y;

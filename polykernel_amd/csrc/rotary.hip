@@ -28,7 +28,7 @@ int check_cache(const char *who, const pk_paged_cache *c, Cache *out) {
 
 int check_batch(const char *who, const pk_paged_batch *b, const pk_paged_cache *c, Batch *out) {
   PK_CHECK_ARG(b, "%s: null batch", who);
-  PK_CHECK_ARG(b->sequences >= 0 && b->tokens >= 0 && b->table_width >= 0 && b->max_q >= 0,
+  PK_CHECK_ARG(b->sequences >= 0 && b->tokens >= 0 && b->table_width >= 0 && b->max_q >= 0 && b->max_kv >= 0,
                "%s: invalid batch (%d sequences, %d tokens, %d pages each)", who, b->sequences, b->tokens, b->table_width);
   PK_CHECK_ARG((b->page_table || b->table_width == 0 || b->sequences == 0) && (b->kv_len || b->sequences == 0),
                "%s: null page_table or kv_len", who);

@@ -376,7 +376,7 @@ def _refuse_paged(k_cache, v_cache, page_table, kv_len, dev: int) -> None:
     raise ValueError("page_table: the pages of a sequence must be contiguous")
 
 
-def _paged(k_cache, v_cache, page_table, q_start, kv_len, tokens: int, max_q: int, dev: int):
+def _paged(k_cache, v_cache, page_table, q_start, kv_len, tokens: int, max_q: int, max_kv: int, dev: int):
     """(cache, heads, dim, batch) for the C entry points, once everything is as it has to be: one
     condition, since a step's call takes no longer than its checks."""
     try:
@@ -397,7 +397,7 @@ def _paged(k_cache, v_cache, page_table, q_start, kv_len, tokens: int, max_q: in
     elif tokens != B:
         raise ValueError(f"q_start: without it every sequence has one token (got {tokens} tokens, {B} sequences)")
     return (_lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), k0, k1, k2, v0, v1, v2, pages, rows, heads, dim), heads,
-            dim, _lib.PagedBatch(page_table.data_ptr(), t0, width, q_start, kv_len.data_ptr(), B, tokens, max_q))
+            dim, _lib.PagedBatch(page_table.data_ptr(), t0, width, q_start, kv_len.data_ptr(), B, tokens, max_q, max_kv))
 
 
 def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -415,7 +415,7 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     behind the last sequence's, and tokens on a page number outside the cache, write nothing.
     `q_out` may be `q`."""
     T, dev = k.shape[0] if isinstance(k, torch.Tensor) and k.dim() == 3 else 0, _device()
-    cache, heads, D, batch = _paged(k_cache, v_cache, page_table, q_start, kv_len, T, 0, dev)
+    cache, heads, D, batch = _paged(k_cache, v_cache, page_table, q_start, kv_len, T, 0, 0, dev)
     kt, vt = _tokens(k, "k", heads, D, T, dev), _tokens(v, "v", heads, D, T, dev)
     rot = None if turns is None else _rotation(turns, interleaved, False, magnitude, dev)
     qt = ot = None
@@ -437,20 +437,21 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
-                    q_start: Optional[torch.Tensor], kv_len: torch.Tensor, *, max_q: Optional[int] = None,
+                    q_start: Optional[torch.Tensor], kv_len: torch.Tensor, *, max_q: Optional[int] = None, max_kv: int = 0,
                     scale: Optional[float] = None, causal: bool = True, window: int = 0,
                     workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of the new tokens q [tokens, q heads, D] over the pages of their sequences
     (arguments as `paged_kv_append`, which comes first).  Query head h reads key head
     h // (q heads / heads).  A token at position p sees the keys up to p (causal) or all kv_len[b],
-    and of them those above p - window (window > 0); one that sees none gets zeros.  `max_q`: the
-    most new tokens of a sequence, as far as known; it is for speed alone.  `out` keeps its rows
+    and of them those above p - window (window > 0); one that sees none gets zeros.  `max_q` and
+    `max_kv`: the most new tokens and the most keys of a sequence, as far as known (0: as many keys
+    as the table reaches); they are for speed alone.  `out` keeps its rows
     behind the last sequence's tokens."""
     T, dev = q.shape[0] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0, _device()
     if max_q is None:
         B = max(kv_len.shape[0], 1) if isinstance(kv_len, torch.Tensor) and kv_len.dim() else 1
         max_q = -(-T // B)
-    cache, _, D, batch = _paged(k_cache, v_cache, page_table, q_start, kv_len, T, max_q, dev)
+    cache, _, D, batch = _paged(k_cache, v_cache, page_table, q_start, kv_len, T, max_q, max_kv, dev)
     qt = _tokens(q, "q", 0, D, T, dev)
     Hq = q.shape[1]
     if out is None:

@@ -110,7 +110,7 @@ def paged_cache(**kw):
 
 def paged_batch(**kw):
     return _lib.PagedBatch(**{**dict(page_table=FAKE, table_stride=4, table_width=4, q_start=FAKE, kv_len=FAKE,
-                                     sequences=2, tokens=2, max_q=1), **kw})
+                                     sequences=2, tokens=2, max_q=1, max_kv=0), **kw})
 
 
 BAD_PAGED = [
@@ -122,6 +122,7 @@ BAD_PAGED = [
     (dict(cache=paged_cache(dim=1025)), "UNSUPPORTED", "1024"),
     (dict(batch=paged_batch(tokens=-1)), "INVALID_ARG", "invalid batch"),
     (dict(batch=paged_batch(max_q=-1)), "INVALID_ARG", "invalid batch"),
+    (dict(batch=paged_batch(max_kv=-1)), "INVALID_ARG", "invalid batch"),
     (dict(batch=paged_batch(kv_len=None)), "INVALID_ARG", "null"),
     (dict(batch=paged_batch(page_table=None)), "INVALID_ARG", "null"),
     (dict(batch=paged_batch(q_start=None, tokens=1)), "INVALID_ARG", "without q_start"),
@@ -201,39 +202,46 @@ def test_front_end_refuses(call, error, word):
 
 
 # ---- which kernels take a call ----------------------------------------------------------
-def attention_plan(q_heads=32, heads=8, dim=128, page_size=16, table_width=64, tokens=1, sequences=1, max_q=1, window=0):
+def attention_plan(q_heads=32, heads=8, dim=128, page_size=16, table_width=64, tokens=1, sequences=1, max_q=1, window=0,
+                   max_kv=0):
     out = _lib.PagedPlan()
     cache = paged_cache(heads=heads, dim=dim, page_size=page_size, pages=1000)
-    batch = paged_batch(table_width=table_width, tokens=tokens, sequences=sequences, max_q=max_q)
+    batch = paged_batch(table_width=table_width, tokens=tokens, sequences=sequences, max_q=max_q, max_kv=max_kv)
     _lib.check(_lib.load().pk_paged_attention_plan(q_heads, cache, batch, window, out), "pk_paged_attention_plan")
-    size = _lib.load().pk_paged_attention_workspace_size(q_heads, cache, batch)
-    if not out.dim or (out.splits <= 1 and (out.whole or out.workgroups <= 1)):
-        assert size == 0 or window
     return out
 
 
 def test_plans():
     p = attention_plan()  # a step on up to 1024 keys
-    assert (p.dim, p.step_rows, p.whole, p.splits) == (128, 16, 0, 0) and 1 < p.workgroups <= 512
+    assert (p.dim, p.whole, p.splits) == (128, 0, 0) and 1 < p.workgroups <= 1024
     p = attention_plan(table_width=20)  # up to 320 keys: items are not cut, and nothing merged
     assert p.whole == 1 and p.workgroups == 8 and p.splits == 0
-    assert attention_plan(q_heads=256, heads=8).step_rows == 32
-    assert attention_plan(q_heads=512, heads=8).step_rows == 64
-    assert attention_plan(q_heads=512, heads=8, dim=256).step_rows == 32
+    assert attention_plan(q_heads=128).splits == 0 and attention_plan(q_heads=136).workgroups == 0  # 16 and 17 rows
     p = attention_plan(tokens=2048, max_q=2048, table_width=512)
-    assert p.step_rows == 0 and p.splits == 1 and p.items == (2048 * 4 // 128 + 1) * 8
+    assert p.workgroups == 0 and p.splits == 1 and p.items == (2048 * 4 // 128 + 1) * 8
     assert attention_plan(tokens=64, max_q=64, table_width=512).splits > 1
     mixed = dict(tokens=600, sequences=40, max_q=500)
     p = attention_plan(**mixed, table_width=512)
-    assert p.step_rows == 16 and p.splits >= 1
-    assert attention_plan(**mixed, table_width=512, window=512).step_rows == 0  # nobody reaches far
-    assert attention_plan(**mixed, table_width=100).step_rows == 0
-    assert attention_plan(tokens=600, sequences=4, max_q=150, table_width=512).step_rows == 0  # all as long as the hint
+    assert p.workgroups > 1 and p.splits >= 1
+    assert attention_plan(**mixed, table_width=512, window=512).workgroups == 0  # nobody reaches far
+    assert attention_plan(**mixed, table_width=90).workgroups == 0
+    assert attention_plan(**mixed, table_width=512, max_kv=1500).workgroups == 0
+    assert attention_plan(tokens=600, sequences=4, max_q=150, table_width=512).workgroups == 0  # all as long as the hint
     for general in (dict(dim=20), dict(dim=320), dict(dim=1024)):
         assert attention_plan(**general).dim == 0
     # a line of steps that a 32-bit place cannot hold goes to the general kernel
-    p = attention_plan(tokens=1 << 20, sequences=1 << 20, table_width=1 << 20, q_heads=64, heads=64)
-    assert p.dim == 0
+    assert attention_plan(tokens=1 << 20, sequences=1 << 20, table_width=1 << 20, q_heads=64, heads=64).dim == 0
+
+
+def test_a_window_needs_no_more_workspace():
+    """The size is asked for without the window."""
+    for tokens in (1, 40, 300, 3000):
+        for width in (30, 100, 1000, 8000):
+            for window in (1, 100, 1000, 5000, 50000):
+                for dim in (64, 96, 256):
+                    a = attention_plan(tokens=tokens, max_q=tokens, table_width=width, dim=dim)
+                    b = attention_plan(tokens=tokens, max_q=tokens, table_width=width, dim=dim, window=window)
+                    assert b.splits <= a.splits and b.workgroups <= a.workgroups and b.items <= a.items and b.whole == a.whole
 
 
 def test_workspace_refused():
