@@ -133,6 +133,9 @@ struct Choice {
 // Runs of keys of the chunk kernel's items: the longest workgroup's steps, a CU's workgroups
 // in so many rounds, against the states that are written and added (66 KB each at D 128).
 // `us`: a step of one workgroup alone on a CU; `shared`: of each more that runs beside it.
+// 8 heads to 32, D 128: 24 sequences of 8 tokens on up to 3000 keys 62 us in one run, 45 in 2
+// (taken), 46 in 4; 512 tokens on 4096 keys 81, 59 and 51 (taken); 1000 on 1000 28 (taken), 39
+// and 41; 128 on 16000 302, 159 and 87, 50 in 16 (taken).
 int chunk_splits(int64_t items, int64_t steps, int dp) {
   const int at_once = dp == 64 ? 4 : dp == 128 ? 2 : 1;
   const double us = dp == 64 ? 0.8 : dp == 128 ? 1.2 : 2.3, shared = dp == 64 ? 0.6 : dp == 128 ? 0.97 : 2.3;
@@ -142,7 +145,7 @@ int chunk_splits(int64_t items, int64_t steps, int dp) {
     const int64_t groups = items * s, per_cu = (groups + 255) / 256;
     const double rounds = (double)((per_cu + at_once - 1) / at_once);
     const double step = std::max(us, shared * std::min<int64_t>(per_cu, at_once));
-    const double time = rounds * (step * ((steps + s - 1) / s) + 3) + (s > 1 ? 3.5 + 0.028 * dp / 128 * groups : 0);
+    const double time = rounds * (step * ((steps + s - 1) / s) + 3) + (s > 1 ? 3.5 + 0.012 * dp / 128 * groups : 0);
     if (time < least) {
       least = time;
       best = s;
@@ -162,7 +165,10 @@ Choice choose(int q_heads, const pk_paged_cache &c, const pk_paged_batch &b, int
   // a hint of fewer tokens than there are on average is none
   const int64_t most = std::max<int64_t>(b.max_q, (b.tokens + B - 1) / B);
   const bool even = (int64_t)b.max_q * B == b.tokens;  // all sequences have the hint's length
-  const bool chunks = most * group > PD_ROWS;
+  // Short runs of few sequences are the step kernel's up to two items for each: 5 tokens on 1000
+  // keys, 8 heads to 32, 11.0 us against 14.0; four sequences of 5 on up to 3000 are not, 22.0 and 19.9.
+  const bool brief = B * c.heads * steps <= 512;
+  const bool chunks = most * group > (brief ? 2 * PD_ROWS : PD_ROWS);
   bool few = !chunks;
   if (chunks) {
     const int64_t items = (b.tokens * group / PC_ROWS + B) * c.heads;
@@ -180,15 +186,20 @@ Choice choose(int q_heads, const pk_paged_cache &c, const pk_paged_batch &b, int
     r.splits = splits;
     // Sequences of few rows beside chunks are the step kernel's, unless all are chunks, or the
     // few cost the chunk kernel less than another launch and merge: 30 tokens beside 2 chunks of
-    // 500, 8 heads to 32, on up to 1000 keys 61 us with both kernels and 55 with one, 2000 91 and
-    // 86, 4000 135 and 144; 60 beside 2048 on 2000 165 and 214; 8 beside 200 on 3000 60 and 47.
+    // 500, 8 heads to 32, on up to 1000 keys 61 us with both kernels and 53 with one, 2000 92 and
+    // 81, 4000 136 and 134; 60 beside 2048 on 2000 187 and 240; 8 beside 200 on 3000 60 and 50.
     few = !(B == 1 || even || B * c.heads * reach <= 8192);
   }
   if (few) {
     // no more workgroups than the tables can have work for
     const int64_t items = (b.tokens * group / PD_ROWS + B) * c.heads;
     if (items > INT32_MAX / steps) return Choice{};  // a line of 2^31 steps or more: the general kernel
-    r.whole = keys <= 6 * PT_STEP;
+    // Items are left whole, and nothing is merged, where their steps are few, or so many items fill
+    // the machine.  8 heads to 32, D 128: 64 sequences of up to 1000 keys 28.5 us whole and 31 cut,
+    // of 2000 54 and 56; 128 at D 64 33 and 47; 16 of 450 12.4 and 13.6, of 700 17.4 and 13.9; 1 of
+    // 200 9.2 and 9.2, of 450 12.7 and 9.7.
+    const int64_t likely = chunks ? B * c.heads : items, most_steps = likely >= 512 ? 34 : likely >= 128 ? 8 : 6;
+    r.whole = keys <= most_steps * PT_STEP;
     r.workers = (int)std::max<int64_t>(1, std::min<int64_t>(256 * pd_groups(dp), r.whole ? items : items * steps));
   }
   r.dp = dp;

@@ -216,7 +216,11 @@ def test_plans():
     assert (p.dim, p.whole, p.splits) == (128, 0, 0) and 1 < p.workgroups <= 1024
     p = attention_plan(table_width=20)  # up to 320 keys: items are not cut, and nothing merged
     assert p.whole == 1 and p.workgroups == 8 and p.splits == 0
-    assert attention_plan(q_heads=128).splits == 0 and attention_plan(q_heads=136).workgroups == 0  # 16 and 17 rows
+    long = dict(table_width=512)
+    assert attention_plan(q_heads=128, **long).splits == 0 and attention_plan(q_heads=136, **long).workgroups == 0  # 16 and 17 rows
+    assert attention_plan(q_heads=256).splits == 0 and attention_plan(q_heads=264).workgroups == 0  # 32 and 33 of a short one
+    assert attention_plan(sequences=64, tokens=64, table_width=125).whole == 1  # many items fill the machine uncut
+    assert attention_plan(sequences=16, tokens=16, table_width=125).whole == 0
     p = attention_plan(tokens=2048, max_q=2048, table_width=512)
     assert p.workgroups == 0 and p.splits == 1 and p.items == (2048 * 4 // 128 + 1) * 8
     assert attention_plan(tokens=64, max_q=64, table_width=512).splits > 1
