@@ -270,7 +270,7 @@ PK_API int launch_paged_kv_append(const pk_tokens *k, const pk_tokens *v, const 
  * does not see, or on pages that are not there, take no part, whatever they
  * hold.  A token that sees no key gets zeros.  Any head dim up to 1024.
  * `workspace` holds pk_paged_attention_workspace_size bytes (0: may be NULL) for
- * the call's partial results. */
+ * the call's partial results; calls that may run at the same time need one each. */
 PK_API size_t pk_paged_attention_workspace_size(int q_heads, const pk_paged_cache *cache, const pk_paged_batch *batch);
 PK_API int launch_paged_attention(const pk_tokens *q, const pk_tokens *out, int q_heads, const pk_paged_cache *cache,
                                   const pk_paged_batch *batch, float scale, int causal, int window, void *workspace,

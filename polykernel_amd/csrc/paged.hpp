@@ -18,6 +18,9 @@ namespace paged {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
+// Workgroups of 256 threads along one side of a grid: its threads are a 32-bit number.
+constexpr int64_t MOST_BLOCKS = INT64_C(0xFFFFFFFF) / 256;
+
 // n / d for 0 <= n < 2^31 by a multiplication: m = ceil(2^(32 + s) / d), s =
 // ceil(log2 d), less 2^32, so that q = (umulhi(n, m) + n) >> s; exact since the
 // error n (m' d - 2^(32 + s)) / (d 2^(32 + s)) stays below 1 / d for n < 2^32

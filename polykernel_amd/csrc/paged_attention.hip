@@ -21,7 +21,7 @@ template <int N>  // dims per lane
 __global__ __launch_bounds__(PG_THREADS) void paged_general_kernel(AttendArgs g) {
   __shared__ float so[PG_WAVES][64 * N], sml[PG_WAVES][2];
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, D = g.cache.dim;
-  const int t = blockIdx.x / g.q_heads, h = blockIdx.x % g.q_heads;
+  const int t = blockIdx.x, h = blockIdx.y;
   const int b = sequence_of(g.batch, t);
   if (b < 0) return;
   const Seq s = sequence(g.batch, b);
@@ -82,9 +82,12 @@ __global__ __launch_bounds__(PG_THREADS) void paged_general_kernel(AttendArgs g)
 }
 
 int run_general(const AttendArgs &g, hipStream_t st) {
-  const int64_t blocks = (int64_t)g.batch.tokens * g.q_heads;
-  const unsigned n = (unsigned)blocks;
   const int D = g.cache.dim;
+  if (g.batch.tokens > MOST_BLOCKS || g.q_heads > 65535) {
+    set_error("launch_paged_attention: %d tokens of %d query heads are not supported", g.batch.tokens, g.q_heads);
+    return PK_ERR_UNSUPPORTED;
+  }
+  const dim3 n(g.batch.tokens, g.q_heads);
   if (D <= 64) paged_general_kernel<1><<<n, PG_THREADS, 0, st>>>(g);
   else if (D <= 128) paged_general_kernel<2><<<n, PG_THREADS, 0, st>>>(g);
   else if (D <= 256) paged_general_kernel<4><<<n, PG_THREADS, 0, st>>>(g);
@@ -181,7 +184,7 @@ Choice choose(int q_heads, const pk_paged_cache &c, const pk_paged_batch &b, int
       reach = std::min<int64_t>(reach, (window + PT_KEYS) / PT_STEP + 2);
       splits = std::min(splits, chunk_splits(likely, reach, dp));
     }
-    if (items * splits > INT32_MAX) return r;
+    if (items * splits > MOST_BLOCKS) return r;
     r.items = (int)items;
     r.splits = splits;
     // Sequences of few rows beside chunks are the step kernel's, unless all are chunks, or the

@@ -90,7 +90,7 @@ __device__ __forceinline__ bool find_item(const ChunkArgs &d, int splits, int i,
   const int x = in_head - it.split * n, turn = total * splits <= 512 ? (n + 1) / 2 : n;
   it.tile = x < turn ? n - 1 - x : x - turn;
   order = at + it.hk * n + it.tile;
-  return order < d.items;
+  return (unsigned)order < (unsigned)d.items;
 }
 
 // The item's first key (of a tile) and its steps.

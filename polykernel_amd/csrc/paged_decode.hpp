@@ -396,7 +396,7 @@ __device__ __forceinline__ void paged_decode_merge_body(const DecodeArgs &d) {
   const size_t stride = pd_part_floats(DP);
   const Cut cut = reinterpret_cast<const Cut *>(d.parts + (size_t)(2 * d.most) * stride)[w];
   const int w0 = cut.first, w1 = cut.last, rows = cut.rows, D = g.cache.dim;
-  if (w0 < 0) return;
+  if (w0 < 0 || w0 >= w || w1 < w) return;  // (the latter two only where q_start goes down)
   const float c2 = fabsf(g.c2);
   const float *p0 = d.parts + (size_t)(2 * w0 + cut.second) * stride;
   int groups = 1;

@@ -267,11 +267,15 @@ int run_rotate(RotateArgs g, int q_heads, int kv_heads, int D, bool wide, const 
   g.of_value = FastDiv((uint32_t)per_value);
   g.of_token = FastDiv((uint32_t)total);
   g.per_group = g.tokens >= 4096 && total <= INT32_MAX / (2 * RO_TOKENS) ? RO_TOKENS : 1;
-  const unsigned blocks = (unsigned)((g.tokens + (int64_t)g.per_group - 1) / g.per_group);
+  const int64_t blocks = (g.tokens + (int64_t)g.per_group - 1) / g.per_group;
+  if (blocks > MOST_BLOCKS) {
+    set_error("%s: %d tokens are not supported", who, g.tokens);
+    return PK_ERR_UNSUPPORTED;
+  }
   const size_t lds = (size_t)g.per_group * g.rot.half * sizeof(float2);
-  if (wide) rotate_kernel<8, APPEND><<<blocks, RO_THREADS, lds, st>>>(g);
-  else rotate_kernel<1, APPEND><<<blocks, RO_THREADS, lds, st>>>(g);
-  PK_LAUNCH_CHECK(who);
+  if (wide) rotate_kernel<8, APPEND><<<(unsigned)blocks, RO_THREADS, lds, st>>>(g);
+  else rotate_kernel<1, APPEND><<<(unsigned)blocks, RO_THREADS, lds, st>>>(g);
+  PK_LAUNCH_CHECK("rotate_kernel");
   return PK_OK;
 }
 
@@ -348,7 +352,7 @@ int launch_rotary(const uint16_t *x, const int64_t *xs, uint16_t *out, const int
   g.of_entry = FastDiv((uint32_t)S);
   g.tokens = (int)tokens;
   const bool wide = aligned16(x) && aligned16(out) && strides8(xs[0], xs[1], xs[2]) && strides8(os[0], os[1], os[2]);
-  return run_rotate<false>(g, H, 0, D, wide, "rotate_kernel", (hipStream_t)stream);
+  return run_rotate<false>(g, H, 0, D, wide, "launch_rotary", (hipStream_t)stream);
 }
 
 int launch_paged_kv_append(const pk_tokens *k, const pk_tokens *v, const pk_tokens *q, const pk_tokens *q_out, int q_heads,
@@ -379,7 +383,7 @@ int launch_paged_kv_append(const pk_tokens *k, const pk_tokens *v, const pk_toke
               strides8(k->token, k->head) && strides8(v->token, v->head) &&
               strides8(cache->k_page, cache->k_head, cache->k_row) && strides8(cache->v_page, cache->v_head, cache->v_row);
   if (q) wide = wide && aligned16(q->data) && aligned16(q_out->data) && strides8(q->token, q->head) && strides8(q_out->token, q_out->head);
-  return run_rotate<true>(g, q_heads, cache->heads, cache->dim, wide, "rotate_kernel", (hipStream_t)stream);
+  return run_rotate<true>(g, q_heads, cache->heads, cache->dim, wide, who, (hipStream_t)stream);
 }
 
 }  // extern "C"

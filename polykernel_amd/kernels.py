@@ -298,6 +298,9 @@ def _table(t: torch.Tensor, shape, dtype: torch.dtype, name: str, dev: int) -> i
     raise ValueError(f"{name}: tensor must be contiguous")
 
 
+_INT = 0x7FFFFFFF  # numbers that the C entry points take in 32 bits (ctypes would cut larger ones)
+
+
 # a result's memory: 1.6 us where torch.empty with a shape, type and device takes 3.7
 def _result(like: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(like, memory_format=torch.contiguous_format)
@@ -315,7 +318,7 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, turns: torch.Tensor, *, int
 
     x is [tokens, heads, D] with positions [tokens], or [B, heads, S, D] with positions [S] or
     [B, S] (int32); any strides with contiguous head dims.  `inverse` rotates back, which is the
-    gradient: dx = rotary(dy, positions, turns, inverse=True).  `out` (contiguous by default) may
+    gradient: dx = rotary(dy, positions, turns, inverse=True) with the same magnitude.  `out` (contiguous by default) may
     be `x`."""
     if not isinstance(x, torch.Tensor) or x.dim() not in (3, 4):
         raise ValueError("x: expected a tensor [tokens, heads, D] or [B, heads, S, D]")
@@ -339,6 +342,8 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, turns: torch.Tensor, *, int
         whole = isinstance(positions, torch.Tensor) and positions.dim() == 2
         per = S if whole else 0
         pos = _table(positions, (B, S) if whole else (S,), torch.int32, "positions", dev)
+    if B * S > _INT or H * D > _INT:
+        raise ValueError(f"x: {B * S} tokens of {H * D} elements (each at most {_INT})")
     rot = _rotation(turns, interleaved, inverse, magnitude, dev)
     check(_lib.load().launch_rotary(x.data_ptr(), _strides3(*xs), out.data_ptr(), _strides3(*os_), pos, per, B, S, H, D,
                                     rot, _stream()), "launch_rotary")
@@ -354,6 +359,8 @@ def _tokens(t: torch.Tensor, name: str, heads: int, dim: int, tokens: int, dev: 
     n, h, d = t.shape
     if n != tokens or d != dim or (heads and h != heads):
         raise ValueError(f"{name}: expected [{tokens}, {heads or 'heads'}, {dim}], got {tuple(t.shape)}")
+    if n > _INT or h > _INT:
+        raise ValueError(f"{name}: {n} tokens of {h} heads (each at most {_INT})")
     return _lib.Tokens(t.data_ptr(), strides[0], strides[1])
 
 
@@ -392,6 +399,8 @@ def _paged(k_cache, v_cache, page_table, q_start, kv_len, tokens: int, max_q: in
         fine = False
     if not fine:
         _refuse_paged(k_cache, v_cache, page_table, kv_len, dev)
+    if pages > _INT:
+        raise ValueError(f"k_cache: {pages} pages (at most {_INT})")
     if q_start is not None:
         q_start = _table(q_start, (B + 1,), torch.int32, "q_start", dev)
     elif tokens != B:
@@ -446,11 +455,14 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     and of them those above p - window (window > 0); one that sees none gets zeros.  `max_q` and
     `max_kv`: the most new tokens and the most keys of a sequence, as far as known (0: as many keys
     as the table reaches); they are for speed alone.  `out` keeps its rows
-    behind the last sequence's tokens."""
+    behind the last sequence's tokens.  A `workspace` holds partial results: calls that may run at
+    the same time need one each."""
     T, dev = q.shape[0] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0, _device()
     if max_q is None:
         B = max(kv_len.shape[0], 1) if isinstance(kv_len, torch.Tensor) and kv_len.dim() else 1
         max_q = -(-T // B)
+    if not (0 <= max_q <= _INT and 0 <= max_kv <= _INT and 0 <= window <= _INT):
+        raise ValueError(f"max_q {max_q}, max_kv {max_kv}, window {window}: each from 0 to {_INT}")
     cache, _, D, batch = _paged(k_cache, v_cache, page_table, q_start, kv_len, T, max_q, max_kv, dev)
     qt = _tokens(q, "q", 0, D, T, dev)
     Hq = q.shape[1]
@@ -466,6 +478,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if workspace is not None:
         if workspace.get_device() != dev:
             raise _elsewhere(workspace, "workspace", dev)
+        if not workspace.is_contiguous():
+            raise ValueError("workspace: tensor must be contiguous")
         ws, room = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     else:
         need = lib.pk_paged_attention_workspace_size(Hq, cache, batch)

@@ -259,7 +259,7 @@ def test_append_leaves_what_is_not_there(pk):
 
 # ---- attention ------------------------------------------------------------------
 def run(pk, qs, kvs, Hq, Hkv, D, P, *, window=0, causal=True, rows_first=False, pad=0, std=1.0, seed=0, scale=None,
-        max_q=None, spoil=None, behind=0, single=False):
+        max_q=None, max_kv=0, spoil=None, behind=0, single=False):
     g = gen(seed + D + P)
     table, pages = layout(g, kvs, P)
     T = sum(qs)
@@ -271,7 +271,7 @@ def run(pk, qs, kvs, Hq, Hkv, D, P, *, window=0, causal=True, rows_first=False, 
         spoil(kc, vc, table)
     out = torch.full((T + behind, Hq, D), 5.0, dtype=BF, device="cuda")
     where = (kc, vc, table, q_start, kv_len)
-    pk.paged_attention(q, *where, max_q=max_q, window=window, causal=causal, scale=scale, out=out)
+    pk.paged_attention(q, *where, max_q=max_q, max_kv=max_kv, window=window, causal=causal, scale=scale, out=out)
     s = scale if scale is not None else 1.0 / math.sqrt(D)
     want, bound = ref.attend(q[:T], kc, vc, table, q_start, kv_len, s, causal, window)
     assert bool((out[T:] == 5.0).all())
@@ -327,11 +327,44 @@ def test_attention_rows_first_and_hints(pk, qs, kvs, Hq, Hkv, D, P):
     assert len(outs) == 5
 
 
-def plan(qs, kvs, Hq, Hkv, D, P, max_q, window=0):
+def plan(qs, kvs, Hq, Hkv, D, P, max_q, window=0, max_kv=0):
     from tests.test_paged_host import attention_plan
 
     return attention_plan(q_heads=Hq, heads=Hkv, dim=D, page_size=P, table_width=-(-max(kvs) // P), tokens=sum(qs),
-                          sequences=len(qs), max_q=max_q, window=window)
+                          sequences=len(qs), max_q=max_q, window=window, max_kv=max_kv)
+
+
+@pytest.mark.parametrize("max_kv", [1, 64, 1500, 10**9])
+@pytest.mark.parametrize("qs,kvs,Hq,Hkv,D,P", [([1] * 40, [1 + 70 * i for i in range(40)], 8, 2, 128, 16),
+                                               ([60, 1, 30], [1700, 900, 30], 8, 2, 64, 16), ([20], [1500], 4, 1, 256, 8)])
+def test_attention_with_wrong_numbers_of_keys(pk, qs, kvs, Hq, Hkv, D, P, max_kv):
+    run(pk, qs, kvs, Hq, Hkv, D, P, std=2.0, max_kv=max_kv)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,P", [(16, 2, 128, 16), (24, 2, 64, 32), (16, 2, 96, 8), (12, 1, 256, 16)])
+def test_many_sequences_of_few_tokens(pk, Hq, Hkv, D, P):
+    """More sequences than a wave has lanes in the chunk kernel; most waves have no rows, and short sequences are not
+    cut where long ones are."""
+    qs = [1 + i % 5 for i in range(90)]
+    kvs = [q + 25 * i for i, q in enumerate(qs)]
+    got = plan(qs, kvs, Hq, Hkv, D, P, 5)
+    assert got.splits > 1 and got.workgroups == 0
+    run(pk, qs, kvs, Hq, Hkv, D, P, std=2.0, max_q=5, behind=1)
+
+
+@pytest.mark.parametrize("whole,kvs", [(1, [1 + 33 * i for i in range(64)]), (0, [1 + 35 * i for i in range(64)])])
+@pytest.mark.parametrize("Hq,Hkv,D,P", [(8, 8, 128, 16), (16, 8, 64, 8)])
+def test_items_cut_and_whole(pk, Hq, Hkv, D, P, whole, kvs):
+    assert plan([1] * 64, kvs, Hq, Hkv, D, P, 1).whole == whole
+    run(pk, [1] * 64, kvs, Hq, Hkv, D, P, std=2.0)
+
+
+@pytest.mark.parametrize("D,P", [(128, 16), (64, 8)])
+def test_two_items_for_a_short_run(pk, D, P):
+    """17 to 32 rows of one short sequence are the step kernel's."""
+    for q in (5, 8):
+        assert plan([q], [900], 8, 2, D, P, q).splits == 0
+        run(pk, [q], [900], 8, 2, D, P, std=2.0)
 
 
 @pytest.mark.parametrize("window", [0, 2200])
@@ -642,6 +675,17 @@ def test_empty_calls(pk):
     assert bool((pk.paged_attention(q, kc[:0], kc[:0], table, i32(0, 1), i32(9)) == 0).all())
     assert bool((pk.paged_attention(q, kc, kc, table[:, :0], i32(0, 1), i32(9)) == 0).all())
     torch.cuda.synchronize()
+
+
+def test_numbers_and_workspaces_refused(pk):
+    q, c = (torch.zeros(*s, dtype=BF, device="cuda") for s in ((4, 2, 64), (3, 2, 16, 64)))
+    where = (c, c, *(torch.zeros(*s, dtype=torch.int32, device="cuda") for s in ((1, 3), (2,), (1,))))
+    for kw in (dict(window=2**32 + 5), dict(max_q=2**31), dict(max_kv=2**40), dict(window=-2**32 + 5)):
+        with pytest.raises(ValueError, match=next(iter(kw))):
+            pk.paged_attention(q, *where, **kw)
+    room = torch.zeros(1 << 22, dtype=torch.uint8, device="cuda")
+    with pytest.raises(ValueError, match="workspace"):
+        pk.paged_attention(q, *where, workspace=room[::2])
 
 
 def test_front_end_refusals(pk):

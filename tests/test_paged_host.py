@@ -97,7 +97,7 @@ def rotary_call(B=1, S=4, H=2, D=64, rot=None, x=FAKE, positions=FAKE, strides=T
     (dict(rot=rotation(dim=0)), "INVALID_ARG", "rotated"), (dict(rot=rotation(turns=None)), "INVALID_ARG", "turns"),
     (dict(x=None), "INVALID_ARG", "null"), (dict(positions=None), "INVALID_ARG", "null"),
     (dict(strides=False), "INVALID_ARG", "null"), (dict(B=65536, S=65536), "INVALID_ARG", "exceeds"),
-    (dict(H=2**25), "INVALID_ARG", "exceeds"),
+    (dict(H=2**25), "INVALID_ARG", "exceeds"), (dict(S=2**27), "UNSUPPORTED", "tokens"),
 ])
 def test_rotary_refused(kw, code, word):
     assert rotary_call(**kw) == getattr(_lib, "PK_ERR_" + code) and word in _lib.last_error()
@@ -152,6 +152,7 @@ def attend_call(cache=paged_cache(), batch=paged_batch(), q=tok(), out=tok(), q_
     (dict(q=tok(), q_out=tok(), rot=rotation(), q_heads=0), "INVALID_ARG", "query heads"),
     (dict(rot=rotation(inverse=1)), "INVALID_ARG", "inverse"), (dict(rot=rotation(dim=66)), "INVALID_ARG", "rotated"),
     (dict(q=tok(), q_out=tok(), rot=rotation(), q_heads=2**26), "INVALID_ARG", "heads"),
+    (dict(batch=paged_batch(tokens=2**27)), "UNSUPPORTED", "tokens"),
 ])
 def test_append_refused(kw, code, word):
     assert append_call(**kw) == getattr(_lib, "PK_ERR_" + code) and word in _lib.last_error()
@@ -162,6 +163,8 @@ def test_append_refused(kw, code, word):
     (dict(q_heads=3), "INVALID_ARG", "query heads"), (dict(q_heads=0), "INVALID_ARG", "query heads"),
     (dict(window=-1), "INVALID_ARG", "window"),
     (dict(batch=paged_batch(tokens=2**20), q_heads=2**12), "INVALID_ARG", "exceeds"),
+    (dict(cache=paged_cache(dim=20), batch=paged_batch(tokens=2**25)), "UNSUPPORTED", "tokens"),
+    (dict(cache=paged_cache(dim=20), q_heads=70000), "UNSUPPORTED", "query heads"),
 ])
 def test_attention_refused(kw, code, word):
     assert attend_call(**kw) == getattr(_lib, "PK_ERR_" + code) and word in _lib.last_error()
