@@ -231,7 +231,7 @@ int run_decode_as(const DecodeArgs &d, hipStream_t st) {
 }
 template <int DP, int DC>
 int run_chunk_as(const ChunkArgs &d, hipStream_t st) {
-  const unsigned blocks = (unsigned)d.items * d.splits;
+  const unsigned blocks = pc_blocks(d.items * d.splits);
   if (d.a.cache.page.d % PT_KEYS == 0) paged_chunk_kernel<DP, DC, true><<<blocks, PC_THREADS, 0, st>>>(d);
   else paged_chunk_kernel<DP, DC, false><<<blocks, PC_THREADS, 0, st>>>(d);
   PK_LAUNCH_CHECK("paged_chunk_kernel");

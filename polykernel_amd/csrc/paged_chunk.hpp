@@ -13,8 +13,9 @@
 // instructions without a branch (two waves of two workgroups on a SIMD fall into step
 // otherwise, and both wait for the matrix unit and then both for the exponentials).
 //
-// Items of one key head run next to each other on one XCD and share its L2.  Few items are also cut into `splits`
-// runs of keys, whose states paged_chunk_merge_kernel adds in order.
+// Four items of one key head at a time run next to each other on one XCD and share its L2; the
+// next four items of the line go to the next XCD, so that long sequences are everybody's.  Few
+// items are also cut into `splits` runs of keys, whose states paged_chunk_merge_kernel adds in order.
 #pragma once
 
 #include "paged_tiles.hpp"
@@ -42,9 +43,12 @@ struct Item {
   int b, hk, tile;
   int split;
 };
+constexpr int PC_RUN = 4;  // items that an XCD takes at a time
+constexpr int pc_blocks(int items) { return (items + 8 * PC_RUN - 1) / (8 * PC_RUN) * (8 * PC_RUN); }
 // Workgroup i's item and split; false behind the last one.  `order`: place of the item
-// on the line of all, for its parts.
-__device__ __forceinline__ bool find_item(const ChunkArgs &d, int splits, int i, bool spread, Item &it, int &order) {
+// on the line of all, for its parts.  `spread`: workgroups i go to XCDs i % 8, else it is the
+// i-th of the line; `pairs`: up to 512 of them run at once, two on a CU.
+__device__ __forceinline__ bool find_item(const ChunkArgs &d, int splits, int i, bool spread, bool pairs, Item &it, int &order) {
   const AttendArgs &g = d.a;
   const int lane = threadIdx.x & 63, B = g.batch.sequences, per = (B + 63) / 64, G = (int)g.group.d;
   auto tiles_of = [&](const Seq &s) __attribute__((always_inline)) {
@@ -62,9 +66,10 @@ __device__ __forceinline__ bool find_item(const ChunkArgs &d, int splits, int i,
   }
   const int incl = wave_scan(mine);
   const int total = min(__builtin_amdgcn_readlane(incl, 63), d.items);  // (more only where q_start goes down)
-  if (total <= 0 || i / splits >= total) return false;
-  const int v = uniform(spread ? xcd_unit(i, total * splits) : i);
+  static_assert(8 * PC_RUN == 32, "the bits of a place");
+  const int v = uniform(spread ? (i & ~31) | (i & 7) << 2 | (i >> 3 & 3) : i);
   const int u = v / splits;  // any place of the item's group: groups are whole runs of splits
+  if (u >= total) return false;
   const uint64_t beyond = __ballot(u < incl);
   if (beyond == 0) return false;
   const int l = __ffsll((unsigned long long)beyond) - 1;
@@ -78,17 +83,25 @@ __device__ __forceinline__ bool find_item(const ChunkArgs &d, int splits, int i,
     if (u < at + n * g.cache.heads) break;
     at += n * g.cache.heads;
   }
-  // a sequence's run: heads, of each the splits, of each the tiles from the last one
-  const int in_seq = v - at * splits, per_head = n * splits;
-  if ((unsigned)in_seq >= (unsigned)(per_head * g.cache.heads)) return false;
+  // a sequence's run: splits, of each the tiles from the last one on, which sees the most keys, in
+  // runs of four by head; in pairs the workgroups from 256 on take them from the other end, so
+  // that long ones share a CU with short
+  const int heads = g.cache.heads, all = n * heads, in_seq = v - at * splits;
+  if ((unsigned)in_seq >= (unsigned)(all * splits)) return false;
   it.b = uniform(b);
-  it.hk = uniform(in_seq / per_head);
-  const int in_head = uniform(in_seq - it.hk * per_head);
-  it.split = uniform(in_head / n);
-  // from the last tile, which sees the most keys, on; where everything runs at once, two
-  // workgroups on a CU, the second half from the first tile on, so that long ones share with short
-  const int x = in_head - it.split * n, turn = total * splits <= 512 ? (n + 1) / 2 : n;
-  it.tile = x < turn ? n - 1 - x : x - turn;
+  it.split = uniform(in_seq / all);
+  const int x = in_seq - it.split * all;
+  const int turn = pairs && total * splits <= 512 ? min(max(256 - (v - x), 0), all) : all;
+  int y = x < turn ? x : all - 1 - (x - turn), t = n & ~(PC_RUN - 1), run = PC_RUN;
+  if (y < t * heads) {
+    t = y / (PC_RUN * heads) * PC_RUN;
+    y -= t * heads;
+  } else {
+    y -= t * heads;
+    run = n - t;
+  }
+  it.hk = uniform(y / run);
+  it.tile = uniform(n - 1 - (t + y - it.hk * run));
   order = at + it.hk * n + it.tile;
   return (unsigned)order < (unsigned)d.items;
 }
@@ -137,7 +150,7 @@ __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
 
   Item it;
   int order;
-  if (!find_item(d, d.splits, blockIdx.x, true, it, order)) return;
+  if (!find_item(d, d.splits, blockIdx.x, true, DP < 256, it, order)) return;
   const Seq s = it.s;
   const int all_rows = s.n * G, row0 = it.tile * PC_ROWS;
   const int rows = min(PC_ROWS, all_rows - row0);
@@ -533,7 +546,7 @@ __device__ __forceinline__ void paged_chunk_merge_body(const ChunkArgs &d) {
   const AttendArgs &g = d.a;
   Item it;
   int order;
-  if (!find_item(d, 1, blockIdx.x, false, it, order)) return;
+  if (!find_item(d, 1, blockIdx.x, false, false, it, order)) return;
   const Seq s = it.s;
   const int G = (int)g.group.d, D = g.cache.dim;
   const int row0 = it.tile * PC_ROWS, rows = min(PC_ROWS, s.n * G - row0);
