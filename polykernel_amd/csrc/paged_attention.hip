@@ -133,22 +133,25 @@ struct Choice {
   }
 };
 
-// Runs of keys of the chunk kernel's items: the longest workgroup's steps, a CU's workgroups
-// in so many rounds, against the states that are written and added (66 KB each at D 128).
-// `us`: a step of one workgroup alone on a CU; `shared`: of each more that runs beside it.
-// 8 heads to 32, D 128: 24 sequences of 8 tokens on up to 3000 keys 62 us in one run, 45 in 2
-// (taken), 46 in 4; 512 tokens on 4096 keys 81, 59 and 51 (taken); 1000 on 1000 28 (taken), 39
-// and 41; 128 on 16000 302, 159 and 87, 50 in 16 (taken).
-int chunk_splits(int64_t items, int64_t steps, int dp) {
+// Runs of keys of the chunk kernel's items: what a workgroup of the longest item takes among
+// those beside it, or, of more than run at once, what a CU takes for all of its own and the end
+// of the last, against the states that are written and added (66 KB each at D 128).  `part`:
+// an item's steps on average, of the longest's.  `us`: a step of one workgroup alone on a CU;
+// `shared`: of each more that runs beside it.
+// 8 heads to 32, D 128: 512 tokens on 4096 keys 79 us in one run, 59 in 2 and 50 in 4 (taken);
+// 1000 on 1000 27 (taken), 36 and 41; 128 on 16000 296, 157 and 86, 50 in 16 (taken); 24
+// sequences of 5 on up to 3000 56, 41, 38 in 3 (taken) and 40.  8 heads to 8: 5 of up to 4000 on
+// up to 9000 345 (taken), 390 and 432.
+int chunk_splits(int64_t items, int64_t steps, double part, int dp) {
   const int at_once = dp == 64 ? 4 : dp == 128 ? 2 : 1;
   const double us = dp == 64 ? 0.8 : dp == 128 ? 1.2 : 2.3, shared = dp == 64 ? 0.6 : dp == 128 ? 0.97 : 2.3;
   int best = 1;
   double least = 1e30;
   for (int s = 1; s <= 32 && (s == 1 || 4 * s <= steps); ++s) {
-    const int64_t groups = items * s, per_cu = (groups + 255) / 256;
-    const double rounds = (double)((per_cu + at_once - 1) / at_once);
-    const double step = std::max(us, shared * std::min<int64_t>(per_cu, at_once));
-    const double time = rounds * (step * ((steps + s - 1) / s) + 3) + (s > 1 ? 3.5 + 0.012 * dp / 128 * groups : 0);
+    const double groups = (double)items * s, per_cu = groups / 256, longest = (double)((steps + s - 1) / s);
+    double time = 3 + (per_cu <= at_once ? std::max(us, shared * std::ceil(per_cu)) * longest
+                                         : (shared * part * longest + 1) * per_cu + 0.4 * us * longest);
+    if (s > 1) time += 3.5 + 0.02 * dp / 128 * groups;
     if (time < least) {
       least = time;
       best = s;
@@ -179,10 +182,12 @@ Choice choose(int q_heads, const pk_paged_cache &c, const pk_paged_batch &b, int
     const int64_t likely = B == 1 || even ? B * ((b.tokens / B * group + PC_ROWS - 1) / PC_ROWS) * c.heads
                                           : (b.tokens * group / PC_ROWS + (B + 1) / 2) * c.heads;
     int64_t reach = keys / PT_STEP + 1;
-    int splits = chunk_splits(likely, reach, dp);
+    // (lengths are taken to be uneven; of one sequence's tokens the first see `most` keys less than the last)
+    auto part = [&](int64_t of) { return B > 1 ? 0.6 : 1 - 0.5 * std::min(1.0, (double)most / (PT_STEP * of)); };
+    int splits = chunk_splits(likely, reach, part(reach), dp);
     if (window > 0) {  // (no more splits than without, which the workspace is for)
       reach = std::min<int64_t>(reach, (window + PT_KEYS) / PT_STEP + 2);
-      splits = std::min(splits, chunk_splits(likely, reach, dp));
+      splits = std::min(splits, chunk_splits(likely, reach, part(reach), dp));
     }
     if (items * splits > MOST_BLOCKS) return r;
     r.items = (int)items;
