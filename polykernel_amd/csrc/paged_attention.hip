@@ -97,17 +97,17 @@ int run_general(const AttendArgs &g, hipStream_t st) {
 }
 
 // ---- the fast kernels (paged_decode.hpp, paged_chunk.hpp) ------------------------
-template <int DP, bool PAGE16>
+template <int DP, int PAGE>
 __global__ __launch_bounds__(PD_THREADS, pd_groups(DP)) void paged_decode_kernel(DecodeArgs d) {
-  paged_decode_body<DP, PAGE16>(d);
+  paged_decode_body<DP, PAGE>(d);
 }
 template <int DP>
 __global__ __launch_bounds__(PD_THREADS) void paged_decode_merge_kernel(DecodeArgs d) {
   paged_decode_merge_body<DP>(d);
 }
-template <int DP, int DC, bool PAGE16>
+template <int DP, int DC, int PAGE>
 __global__ __launch_bounds__(PC_THREADS, DP == 256 ? 1 : DP == 64 ? 4 : 2) void paged_chunk_kernel(ChunkArgs d) {
-  paged_chunk_body<DP, DC, PAGE16>(d);
+  paged_chunk_body<DP, DC, PAGE>(d);
 }
 template <int DP, int DC>
 __global__ __launch_bounds__(PC_THREADS) void paged_chunk_merge_kernel(ChunkArgs d) {
@@ -225,8 +225,10 @@ bool tile_operands(const AttendArgs &g) {
 
 template <int DP>
 int run_decode_as(const DecodeArgs &d, hipStream_t st) {
-  if (d.a.cache.page.d % PT_KEYS == 0) paged_decode_kernel<DP, true><<<d.most, PD_THREADS, 0, st>>>(d);
-  else paged_decode_kernel<DP, false><<<d.most, PD_THREADS, 0, st>>>(d);
+  const uint32_t page = d.a.cache.page.d;
+  if (page % 16 == 0) paged_decode_kernel<DP, 16><<<d.most, PD_THREADS, 0, st>>>(d);
+  else if (page % 8 == 0) paged_decode_kernel<DP, 8><<<d.most, PD_THREADS, 0, st>>>(d);
+  else paged_decode_kernel<DP, 1><<<d.most, PD_THREADS, 0, st>>>(d);
   PK_LAUNCH_CHECK("paged_decode_kernel");
   if (d.most > 1 && !d.whole) {
     paged_decode_merge_kernel<DP><<<d.most - 1, PD_THREADS, 0, st>>>(d);
@@ -237,8 +239,10 @@ int run_decode_as(const DecodeArgs &d, hipStream_t st) {
 template <int DP, int DC>
 int run_chunk_as(const ChunkArgs &d, hipStream_t st) {
   const unsigned blocks = pc_blocks(d.items * d.splits);
-  if (d.a.cache.page.d % PT_KEYS == 0) paged_chunk_kernel<DP, DC, true><<<blocks, PC_THREADS, 0, st>>>(d);
-  else paged_chunk_kernel<DP, DC, false><<<blocks, PC_THREADS, 0, st>>>(d);
+  const uint32_t page = d.a.cache.page.d;
+  if (page % 16 == 0) paged_chunk_kernel<DP, DC, 16><<<blocks, PC_THREADS, 0, st>>>(d);
+  else if (page % 8 == 0) paged_chunk_kernel<DP, DC, 8><<<blocks, PC_THREADS, 0, st>>>(d);
+  else paged_chunk_kernel<DP, DC, 1><<<blocks, PC_THREADS, 0, st>>>(d);
   PK_LAUNCH_CHECK("paged_chunk_kernel");
   if (d.splits > 1) {
     paged_chunk_merge_kernel<DP, DC><<<dim3(d.items, PC_MERGE), PC_THREADS, 0, st>>>(d);

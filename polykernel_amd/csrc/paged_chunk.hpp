@@ -132,10 +132,11 @@ struct ChunkShape {
 };
 
 // DP: dims of a row in LDS; DC: dims that the products take (head dims up to DC).
-template <int DP, int DC, bool PAGE16>
+template <int DP, int DC, int PAGE>
 __device__ __forceinline__ void paged_chunk_body(const ChunkArgs &d) {
   using S = ChunkShape<DP>;
-  using Tiles = TileLoader<DP, PAGE16, false>;
+  using Tiles = TileLoader<DP, PAGE, false>;
+  constexpr bool PAGE16 = PAGE == 16;
   constexpr int CH = DP / 8, TB = S::TB, SL = S::SL, NI = Tiles::NI, DS = DC / 16, DB = DC / 32, RB = DP * 2;
   static_assert(DC <= DP && DC % 32 == 0, "dims");
   constexpr int KO = DS < 8 ? DS : 8, VO = DB < 4 ? DB : 4;  // lane offsets; dims from 128 on lie 256 bytes further

@@ -16,8 +16,8 @@
 // are read, its values likewise.  Short rings and many workgroups on a CU keep as many
 // bytes in flight as long rings and few, and hide each other's beginnings and ends.  A tile of a page size that is a multiple of 16 lies in one
 // page: its base address is a buffer resource whose length ends the tile at the last
-// key, so rows behind it read as zero and stale pages never reach a product.  Other
-// page sizes look up a page per row and point rows that are not there at zeros.
+// key, so rows behind it read as zero and stale pages never reach a product.  Page sizes that
+// are no multiple of 8 look up a page per row and point rows that are not there at zeros.
 //
 // Work: the steps (64 keys of an item, 16 per wave) of all items lie on one line,
 // which the workgroups cut into equal parts whatever the sequences' lengths; each
@@ -140,7 +140,7 @@ __device__ __forceinline__ bool find_place(const DecodeArgs &d, int w, Place &p)
 
 template <int DP>
 struct DecodeShape {
-  static constexpr int NI = TileLoader<DP, true, true>::NI, TB = TileLoader<DP, true, true>::BYTES;
+  static constexpr int NI = TileLoader<DP, 16, true>::NI, TB = TileLoader<DP, 16, true>::BYTES;
   static constexpr int SL = DP == 64 ? 2 : 1;      // tiles of a ring
   static constexpr int PS = DP + 4;                // row stride of a state in LDS, floats
   static constexpr int STATE = PD_ROWS * PS * 4;   // a wave's sums, then (maximum, sum) of its rows
@@ -148,7 +148,7 @@ struct DecodeShape {
 };
 constexpr int pd_groups(int DP) { return DP == 256 ? 2 : 4; }  // workgroups on a CU
 
-template <int DP, bool PAGE16>
+template <int DP, int PAGE>
 __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
   using S = DecodeShape<DP>;
   constexpr int CH = DP / 8, NI = S::NI, TB = S::TB, SL = S::SL, PS = S::PS, KS = DP / 32, DB = DP / 16;
@@ -173,7 +173,7 @@ __device__ __forceinline__ void paged_decode_body(const DecodeArgs &d) {
     return;
   }
 
-  TileLoader<DP, PAGE16, true> tiles(g);
+  TileLoader<DP, PAGE, true> tiles(g);
   int u = at.first, in_seq = at.in_seq, b = at.b;
   bool first_segment = true;
   while (u < at.last && b < g.batch.sequences) {

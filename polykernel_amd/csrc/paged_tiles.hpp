@@ -78,12 +78,16 @@ __device__ __forceinline__ void dma_lds16_at(const void *src, uint32_t lds) {
 //
 // A page size that is a multiple of 16 holds a tile in one page (PAGE16): its address is a
 // buffer resource whose length ends the tile, so nothing is computed per lane; 64 tiles'
-// pages are looked up at a time, a lane each.  Other sizes look up a page per row, 4 tiles
-// at a time, and lanes without a row read zeros.  NT: read once, non-temporal.
-template <int DP, bool PAGE16, bool NT>
+// pages are looked up at a time, a lane each.  Multiples of 8 have a resource for each half
+// of the tile (one token of 2 sequences on up to 46000 keys, 2 heads to 6 of 80, in pages of
+// 8: 23 us, by rows 27, in pages of 16 18).  Other sizes look up a page per row, 4 tiles at a
+// time, every lane has its own address, and lanes without a row read zeros.
+// PAGE: what the page size is a multiple of: 16, 8 or 1.  NT: read once, non-temporal.
+template <int DP, int PAGE, bool NT>
 struct TileLoader {
+  static constexpr bool PAGE16 = PAGE == 16;
   static constexpr int CH = DP / 8, RPI = 1024 / (2 * DP), NI = PT_KEYS / RPI, BYTES = PT_KEYS * DP * 2;
-  static constexpr int BATCH = PAGE16 ? 64 : 4;
+  static constexpr int PARTS = PT_KEYS / PAGE, BATCH = 64 / PARTS;  // look-ups of a tile, tiles of a look-up
   uint32_t kvo[NI], vvo[NI];
   const uint16_t *kbase, *vbase;
   int b, key0, count, hi;
@@ -103,7 +107,7 @@ struct TileLoader {
   }
   __device__ __forceinline__ int look_up(const AttendArgs &g, int t) const {
     const int lane = threadIdx.x & 63;
-    const int key = key0 + (PAGE16 ? (t + lane) * PT_STEP : (t + (lane >> 4)) * PT_STEP + (lane & 15));
+    const int key = key0 + (t + lane / PARTS) * PT_STEP + lane % PARTS * PAGE;
     return key < hi ? page_of(g.batch, g.cache, b, key) : -1;
   }
   __device__ __forceinline__ void begin(const AttendArgs &g, int b_, int hk, int key0_, int count_, int hi_) {
@@ -122,16 +126,19 @@ struct TileLoader {
     if (t % BATCH == 0 && t > 0 && t < count) vpages = look_up(g, t);
     load(g, t, vpages, vbase, g.cache.v_page, g.cache.v_row, vvo, [](int i) { return v_chunk(i); }, to);
   }
-  // `n` rows from row `row` of a page (none: a resource of no length).
+  // The tile's rows from FROM on, `n` of them from row `row` of a page (none: a resource of no
+  // length), to row TO of the tile.  The resource begins where row 0 of the tile would be.
+  template <int FROM = 0, int TO = PT_KEYS>
   __device__ __forceinline__ static void load_rows(const AttendArgs &g, int page, int row, int n, const uint16_t *base,
                                                    int64_t page_stride, int64_t row_stride, const uint32_t (&offset)[NI],
                                                    uint32_t to) {
-    const uint64_t p = reinterpret_cast<uint64_t>(base) + 2 * (uint64_t)(uint32_t)page * (uint64_t)page_stride +
-                       (uint32_t)row * (uint32_t)(2 * row_stride);
+    uint64_t p = reinterpret_cast<uint64_t>(base) + 2 * (uint64_t)(uint32_t)page * (uint64_t)page_stride +
+                 (uint32_t)row * (uint32_t)(2 * row_stride);
+    if constexpr (FROM > 0) p -= (uint32_t)(2 * FROM * row_stride);
     const pk_u32x4 rs = {(uint32_t)uniform((int)(uint32_t)p), (uint32_t)uniform((int)((uint32_t)(p >> 32) & 0xFFFFu)),
-                         (uint32_t)uniform(n > 0 ? ((n - 1) * (int)row_stride + g.cache.dim) * 2 : 0), 0x00020000u};
+                         (uint32_t)uniform(n > 0 ? ((FROM + n - 1) * (int)row_stride + g.cache.dim) * 2 : 0), 0x00020000u};
 #pragma unroll
-    for (int i = 0; i < NI; ++i) dma_lds16_to<NT>(rs, (uint32_t)uniform((int)to + i * 1024), offset[i]);
+    for (int i = FROM / RPI; i < TO / RPI; ++i) dma_lds16_to<NT>(rs, (uint32_t)uniform((int)to + i * 1024), offset[i]);
   }
   template <typename Chunk>
   __device__ __forceinline__ void load(const AttendArgs &g, int t, int pages, const uint16_t *base, int64_t page_stride,
@@ -141,11 +148,18 @@ struct TileLoader {
       const int page = __builtin_amdgcn_readlane(pages, t % BATCH), n = page < 0 ? 0 : min(PT_KEYS, left);
       const int row = n > 0 ? key - (int)(g.cache.page.div(key) * g.cache.page.d) : 0;
       load_rows(g, n > 0 ? page : 0, row, n, base, page_stride, row_stride, offset, to);
+    } else if constexpr (PAGE == 8) {
+      const int p0 = __builtin_amdgcn_readlane(pages, t % BATCH * 2), p1 = __builtin_amdgcn_readlane(pages, t % BATCH * 2 + 1);
+      const int n0 = p0 < 0 ? 0 : min(8, left), n1 = p1 < 0 ? 0 : min(8, left - 8);
+      const int row0 = n0 > 0 ? key - (int)(g.cache.page.div(key) * g.cache.page.d) : 0;
+      const int row1 = n1 > 0 ? key + 8 - (int)(g.cache.page.div(key + 8) * g.cache.page.d) : 0;
+      load_rows<0, 8>(g, n0 > 0 ? p0 : 0, row0, n0, base, page_stride, row_stride, offset, to);
+      load_rows<8, 16>(g, n1 > 0 ? p1 : 0, row1, n1, base, page_stride, row_stride, offset, to);
     } else {
       const uint16_t *src[NI];
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const int row = row_of(i), page = __shfl(pages, (t % BATCH) * 16 + row, 64);
+        const int row = row_of(i), page = __shfl(pages, (t % BATCH) * PARTS + row / PAGE, 64);
         const bool is = row < left && page >= 0 && 8 * chunk(i) < g.cache.dim;
         const int at = is ? key + row - (int)(g.cache.page.div(key + row) * g.cache.page.d) : 0;
         src[i] = is ? base + page * page_stride + at * row_stride + 8 * chunk(i) : reinterpret_cast<const uint16_t *>(pd_zeros);
@@ -157,7 +171,9 @@ struct TileLoader {
   // Which keys of tile t (the last one of K issued) are on pages that are there, a bit each.
   __device__ __forceinline__ uint32_t there(int t) const {
     if constexpr (PAGE16) return __builtin_amdgcn_readlane(kpages, t % BATCH) < 0 ? 0u : 0xFFFFu;
-    else return (uint32_t)(__ballot(kpages >= 0) >> (16 * (t % BATCH))) & 0xFFFFu;
+    const uint32_t is = (uint32_t)(__ballot(kpages >= 0) >> (PARTS * (t % BATCH)));
+    if constexpr (PAGE == 8) return (is & 1 ? 0xFFu : 0u) | (is & 2 ? 0xFF00u : 0u);
+    else return is & 0xFFFFu;
   }
 };
 

@@ -400,6 +400,22 @@ def test_chunks_cut_along_their_keys(pk, q, kv, D, P):
     run(pk, [q], [kv], 4, 1, D, P, std=2.0, max_q=q, window=700)
 
 
+@pytest.mark.parametrize("gone", [False, True])
+@pytest.mark.parametrize("P", [1, 4, 8, 12, 20, 24, 40])
+@pytest.mark.parametrize("qs,kvs,Hq,Hkv,D", [([1, 3, 1], [3000, 70, 801], 8, 2, 128), ([1, 1], [2500, 9], 4, 1, 64),
+                                             ([1], [1700], 4, 2, 256), ([300, 20], [2100, 700], 6, 1, 64),
+                                             ([150], [1500], 4, 2, 96)])
+def test_page_sizes_that_end_inside_a_tile(pk, qs, kvs, Hq, Hkv, D, P, gone):
+    """With long runs of keys, pages that are not there and no numbers on the rows behind the keys."""
+    def spoil(kc, vc, table):
+        for b, n in enumerate(kvs):
+            if n % P:
+                kc[int(table[b, n // P]), :, n % P:], vc[int(table[b, n // P]), :, n % P:] = float("nan"), float("nan")
+            table[b, 1:n // P:7] = -1 - b
+
+    run(pk, qs, kvs, Hq, Hkv, D, P, std=2.0, spoil=spoil if gone else None)
+
+
 @pytest.mark.parametrize("window", [1, 2, 16, 63, 64, 200, 100000])
 @pytest.mark.parametrize("qs,kvs,Hq,Hkv,D,P", [([1, 1, 1], [1, 70, 1000], 8, 2, 128, 16),
                                                ([5, 2], [300, 40], 8, 2, 64, 32),
