@@ -204,9 +204,11 @@ Choice choose(int q_heads, const pk_paged_cache &c, const pk_paged_batch &b, int
     if (items > INT32_MAX / steps) return Choice{};  // a line of 2^31 steps or more: the general kernel
     // Items are left whole, and nothing is merged, where their steps are few, or so many items fill
     // the machine.  8 heads to 32, D 128: 64 sequences of up to 1000 keys 28.5 us whole and 31 cut,
-    // of 2000 54 and 56; 128 at D 64 33 and 47; 16 of 450 12.4 and 13.6, of 700 17.4 and 13.9; 1 of
-    // 200 9.2 and 9.2, of 450 12.7 and 9.7.
-    const int64_t likely = chunks ? B * c.heads : items, most_steps = likely >= 512 ? 34 : likely >= 128 ? 8 : 6;
+    // of 2000 54 and 56; 128 at D 64 33 and 47; 16 of 500 13.9 and 15.4, of 700 17.4 and 13.9; 1 of
+    // 250 9.2 and 9.6, of 350 11.0 and 9.8.  At D 256, 4 heads to 16, 1 of 180 11.1 and 11.3, of 250
+    // 12.4 and 11.2.
+    const int64_t likely = chunks ? B * c.heads : items;
+    const int64_t most_steps = likely >= 512 ? 34 : likely >= 128 ? 8 : dp == 256 ? 3 : 5;
     r.whole = keys <= most_steps * PT_STEP;
     r.workers = (int)std::max<int64_t>(1, std::min<int64_t>(256 * pd_groups(dp), r.whole ? items : items * steps));
   }
