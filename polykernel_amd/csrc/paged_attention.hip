@@ -15,10 +15,14 @@ namespace paged {
 namespace {
 
 // Any head dim, stride and alignment: a workgroup per token and query head, its waves
-// on every fourth key, a lane on dims lane, lane + 64, ...; states merged in LDS.
-constexpr int PG_WAVES = 4, PG_THREADS = PG_WAVES * 64;
+// on KEYS of every 8 KEYS keys, a lane on dims lane, lane + 64, ...; states merged in LDS.
+// Bound by the chain from a page's number to the sum over the wave, which KEYS keys go
+// through together: a token of 8 sequences on 1000 keys, 2 heads to 8 of 100, 49 us (one key at
+// a time and half the waves 199), at head dim 512 246.
+constexpr int PG_WAVES = 8, PG_THREADS = PG_WAVES * 64;
 template <int N>  // dims per lane
 __global__ __launch_bounds__(PG_THREADS) void paged_general_kernel(AttendArgs g) {
+  constexpr int KEYS = N <= 4 ? 8 : 32 / N;
   __shared__ float so[PG_WAVES][64 * N], sml[PG_WAVES][2];
   const int lane = threadIdx.x & 63, wid = threadIdx.x >> 6, D = g.cache.dim;
   const int t = blockIdx.x, h = blockIdx.y;
@@ -36,25 +40,51 @@ __global__ __launch_bounds__(PG_THREADS) void paged_general_kernel(AttendArgs g)
     q[i] = lane + 64 * i < D ? bf2f(qp[lane + 64 * i]) : 0.f;
     acc[i] = 0.f;
   }
-  for (int j = lo + wid; j < hi; j += PG_WAVES) {
-    const int page = page_of(g.batch, g.cache, b, j);
-    if (page < 0) continue;
-    const int row = j - (int)(g.cache.page.div(j) * g.cache.page.d);
-    const uint16_t *kr = kp + page * g.cache.k_page + row * g.cache.k_row;
-    const uint16_t *vr = vp + page * g.cache.v_page + row * g.cache.v_row;
-    float sc = 0.f;
+  for (int j0 = lo + wid * KEYS; j0 < hi; j0 += PG_WAVES * KEYS) {
+    const uint16_t *kr[KEYS], *vr[KEYS];  // keys that are not there read the query, and take no part
+    bool is[KEYS];
+    float sc[KEYS];
+#pragma unroll
+    for (int u = 0; u < KEYS; ++u) {
+      const int j = j0 + u, page = j < hi ? page_of(g.batch, g.cache, b, j) : -1;
+      const int row = j - (int)(g.cache.page.div(j) * g.cache.page.d);
+      is[u] = page >= 0;
+      kr[u] = is[u] ? kp + page * g.cache.k_page + row * g.cache.k_row : qp;
+      vr[u] = is[u] ? vp + page * g.cache.v_page + row * g.cache.v_row : qp;
+      sc[u] = 0.f;
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (lane + 64 * i < D) sc = fmaf(q[i], bf2f(kr[lane + 64 * i]), sc);
-    sc = wave_sum(sc) * g.c2;
-    const float m_new = fmaxf(m, sc);
+      if (lane + 64 * i < D) {
+#pragma unroll
+        for (int u = 0; u < KEYS; ++u) sc[u] = fmaf(q[i], bf2f(kr[u][lane + 64 * i]), sc[u]);
+      }
+    float m_new = m;
+#pragma unroll
+    for (int u = 0; u < KEYS; ++u) {
+      const float sum = wave_sum(sc[u]) * g.c2;
+      sc[u] = is[u] ? sum : -INFINITY;
+      m_new = fmaxf(m_new, sc[u]);
+    }
     const float mu = m_new == -INFINITY ? 0.f : m_new;
-    const float alpha = __builtin_amdgcn_exp2f(m - mu), p = __builtin_amdgcn_exp2f(sc - mu);
+    const float alpha = __builtin_amdgcn_exp2f(m - mu);
     m = m_new;
-    l = fmaf(l, alpha, p);
+    l *= alpha;
+#pragma unroll
+    for (int u = 0; u < KEYS; ++u) {
+      sc[u] = __builtin_amdgcn_exp2f(sc[u] - mu);
+      l += sc[u];
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (lane + 64 * i < D) acc[i] = fmaf(acc[i], alpha, p * bf2f(vr[lane + 64 * i]));
+      if (lane + 64 * i < D) {
+        acc[i] *= alpha;
+#pragma unroll
+        for (int u = 0; u < KEYS; ++u) {
+          const float v = bf2f(vr[u][lane + 64 * i]);
+          acc[i] = fmaf(sc[u], is[u] ? v : 0.f, acc[i]);
+        }
+      }
   }
 #pragma unroll
   for (int i = 0; i < N; ++i) so[wid][lane + 64 * i] = acc[i];
@@ -83,7 +113,7 @@ __global__ __launch_bounds__(PG_THREADS) void paged_general_kernel(AttendArgs g)
 
 int run_general(const AttendArgs &g, hipStream_t st) {
   const int D = g.cache.dim;
-  if (g.batch.tokens > MOST_BLOCKS || g.q_heads > 65535) {
+  if (2 * (int64_t)g.batch.tokens > MOST_BLOCKS || g.q_heads > 65535) {
     set_error("launch_paged_attention: %d tokens of %d query heads are not supported", g.batch.tokens, g.q_heads);
     return PK_ERR_UNSUPPORTED;
   }
@@ -91,6 +121,7 @@ int run_general(const AttendArgs &g, hipStream_t st) {
   if (D <= 64) paged_general_kernel<1><<<n, PG_THREADS, 0, st>>>(g);
   else if (D <= 128) paged_general_kernel<2><<<n, PG_THREADS, 0, st>>>(g);
   else if (D <= 256) paged_general_kernel<4><<<n, PG_THREADS, 0, st>>>(g);
+  else if (D <= 512) paged_general_kernel<8><<<n, PG_THREADS, 0, st>>>(g);
   else paged_general_kernel<16><<<n, PG_THREADS, 0, st>>>(g);
   PK_LAUNCH_CHECK("paged_general_kernel");
   return PK_OK;

