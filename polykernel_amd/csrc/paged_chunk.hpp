@@ -2,8 +2,9 @@
 //
 // What bounds it: the matrix units and, beside them, the exponentials: 2048 tokens behind
 // 6144 keys, 8 heads to 32 of 128, 0.24 TFLOP in 224 to 240 us, 1000 to 1070 TFLOP/s, the
-// matrix units at work on half of the cycles.  128 rows (token, query head of the group) of one sequence and key head are a workgroup's item, 32 per
-// wave, over steps of 64 keys that the four waves share through LDS.  S^T = K Q^T and
+// matrix units at work on half of the cycles.  128 rows (token, query head of the group) of
+// one sequence and key head are a workgroup's item, 32 per wave, over steps of 64 keys that
+// the four waves share through LDS.  S^T = K Q^T and
 // O^T = V^T P^T run on v_mfma_f32_32x32x16_bf16 as in the contiguous flash kernel: a lane
 // owns one row and half of the keys, so P never leaves its registers.  P is rounded to
 // bf16 once (half a step, 2^-8 of a weight; the second product of a low half would be a

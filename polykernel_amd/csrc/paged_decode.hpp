@@ -3,8 +3,9 @@
 // What bounds it: keys and values are read once for the G query heads that share
 // them (and the few new tokens), so the time is that of streaming them from HBM: 64
 // sequences with 281000 keys in all, 8 heads to 32 of 128, 1.15 GB in 190 us, 6.0 TB/s;
-// the matrix units work on a tenth of the cycles.  Few short sequences are bound by the chain from a page's number to its keys to the sums: 6.7 us
-// for up to 64 keys, 0.85 for each 64 more of an item.
+// the matrix units work on a tenth of the cycles.  Few short sequences are bound by the
+// chain from a page's number to its keys to the sums: 6.7 us for up to 64 keys, 0.85 for
+// each 64 more of an item.
 //
 // A row is a (token, query head of the group) pair; 16 rows of one sequence and key
 // head are one item.  Both products run on the matrix units, transposed: S^T =

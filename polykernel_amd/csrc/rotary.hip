@@ -34,8 +34,9 @@ int check_batch(const char *who, const pk_paged_batch *b, const pk_paged_cache *
                "%s: null page_table or kv_len", who);
   PK_CHECK_ARG(b->q_start || b->tokens >= b->sequences,
                "%s: without q_start every sequence has a token (%d tokens, %d sequences)", who, b->tokens, b->sequences);
-  PK_CHECK_ARG((int64_t)b->table_width * c->page_size <= INT32_MAX - 1023,
-               "%s: %d pages of %d rows: positions are within 1023 of INT32_MAX", who, b->table_width, c->page_size);
+  // (a wave looks up the pages of 64 tiles, of which the last may lie behind all keys)
+  PK_CHECK_ARG((int64_t)b->table_width * c->page_size <= INT32_MAX - 65535,
+               "%s: %d pages of %d rows: positions are within 65535 of INT32_MAX", who, b->table_width, c->page_size);
   *out = Batch{b->page_table, b->q_start,     b->kv_len,    b->table_stride,
                b->sequences,  b->tokens,      b->table_width * c->page_size};
   return PK_OK;

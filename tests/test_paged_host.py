@@ -127,6 +127,7 @@ BAD_PAGED = [
     (dict(batch=paged_batch(page_table=None)), "INVALID_ARG", "null"),
     (dict(batch=paged_batch(q_start=None, tokens=1)), "INVALID_ARG", "without q_start"),
     (dict(batch=paged_batch(table_width=2**27)), "INVALID_ARG", "INT32_MAX"),
+    (dict(batch=paged_batch(table_width=2**27 - 256)), "INVALID_ARG", "INT32_MAX"),
     (dict(batch=None), "INVALID_ARG", "null batch"),
     (dict(cache=None), "INVALID_ARG", "null cache"),
 ]
