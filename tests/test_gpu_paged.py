@@ -526,6 +526,36 @@ def test_attention_strides_and_alignment(pk, qs, kvs, offset, pad):
     ok(out, want, bound)
 
 
+@pytest.mark.parametrize("D", [8, 16, 40, 136, 200, 248])
+@pytest.mark.parametrize("qs,kvs", [([1, 2], [400, 33]), ([70], [300])])
+def test_head_dims_that_fill_no_tile(pk, qs, kvs, D):
+    run(pk, qs, kvs, 6, 2, D, 16, std=2.0, behind=1)
+
+
+@pytest.mark.parametrize("D", [64, 128, 20])
+@pytest.mark.parametrize("qs,kvs", [([1] * 1000, [1 + i % 97 for i in range(1000)]),
+                                    ([3] * 300, [3 + i % 211 for i in range(300)]),
+                                    ([0] * 500 + [40] + [0] * 499, [9] * 500 + [200] + [0] * 499)])
+def test_very_many_sequences(pk, qs, kvs, D):
+    run(pk, qs, kvs, 8, 1, D, 16, max_q=max(qs))
+
+
+@pytest.mark.parametrize("D", [128, 20])
+@pytest.mark.parametrize("n,single", [(1, True), (5, False), (60, False)])
+def test_sequences_that_share_pages(pk, n, single, D):
+    """One table for all sequences (a stride of 0), and caches whose strides differ."""
+    g = gen(21)
+    B, Hq, Hkv, P, kv = 5, 8, 2, 16, 333
+    table, pages = layout(g, [kv], P)
+    table = table.expand(B, -1)
+    kc, vc = cache(g, pages, Hkv, P, D, rows_first=True, pad=8), cache(g, pages, Hkv, P, D)
+    q, kv_len = normal(g, B * n, Hq, D), torch.tensor([kv, 60, 200, 111, 300], dtype=torch.int32, device="cuda")
+    q_start = None if single else starts([n] * B)
+    out = pk.paged_attention(q, kc, vc, table, q_start, kv_len, max_q=n)
+    want, bound = ref.attend(q, kc, vc, table, starts([n] * B), kv_len, 1 / math.sqrt(D))
+    ok(out, want, bound)
+
+
 def test_offsets_past_32_bits(pk):
     """Caches of over 2^32 elements whose far pages are used, by append and attention."""
     Hkv, P, D, Hq = 4, 64, 128, 8
