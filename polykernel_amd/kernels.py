@@ -10,6 +10,7 @@ raises PolyKernelError with the library's message.
 from __future__ import annotations
 
 import math
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -306,9 +307,9 @@ def _result(like: torch.Tensor) -> torch.Tensor:
     return torch.empty_like(like, memory_format=torch.contiguous_format)
 
 
-def _rotation(turns: torch.Tensor, interleaved: bool, inverse: bool, magnitude: float, dev: int) -> _lib.Rotary:
+def _rotation(turns: torch.Tensor, interleaved: bool, inverse: bool, magnitude: float, dev: int) -> bytes:
     n = turns.numel() if isinstance(turns, torch.Tensor) else 0
-    return _lib.Rotary(_table(turns, (n,), torch.float64, "turns", dev), 2 * n, interleaved, inverse, magnitude)
+    return _lib.Rotary.pack(_table(turns, (n,), torch.float64, "turns", dev), 2 * n, interleaved, inverse, magnitude)
 
 
 def rotary(x: torch.Tensor, positions: torch.Tensor, turns: torch.Tensor, *, interleaved: bool = False,
@@ -350,18 +351,23 @@ def rotary(x: torch.Tensor, positions: torch.Tensor, turns: torch.Tensor, *, int
     return out
 
 
-_strides3 = _lib.I64 * 3
+_strides3 = struct.Struct("qqq").pack
 
 
-def _tokens(t: torch.Tensor, name: str, heads: int, dim: int, tokens: int, dev: int) -> _lib.Tokens:
+def _tokens(t: torch.Tensor, name: str, heads: int, dim: int, tokens: int, dev: int) -> bytes:
     """A [tokens, heads, dim] tensor (heads 0: any number)."""
-    strides = _heads(t, 3, name, dev)
-    n, h, d = t.shape
+    try:
+        (token, head, last), (n, h, d) = t.stride(), t.shape
+        fine = t.dtype is bf16 and t.get_device() == dev and (last == 1 or d <= 1)
+    except (AttributeError, ValueError):
+        fine = False
+    if not fine:
+        _heads(t, 3, name, dev)  # says what is wrong
     if n != tokens or d != dim or (heads and h != heads):
         raise ValueError(f"{name}: expected [{tokens}, {heads or 'heads'}, {dim}], got {tuple(t.shape)}")
     if n > _INT or h > _INT:
         raise ValueError(f"{name}: {n} tokens of {h} heads (each at most {_INT})")
-    return _lib.Tokens(t.data_ptr(), strides[0], strides[1])
+    return _lib.Tokens.pack(t.data_ptr(), token, head)
 
 
 def _refuse_paged(k_cache, v_cache, page_table, kv_len, dev: int) -> None:
@@ -405,8 +411,8 @@ def _paged(k_cache, v_cache, page_table, q_start, kv_len, tokens: int, max_q: in
         q_start = _table(q_start, (B + 1,), torch.int32, "q_start", dev)
     elif tokens != B:
         raise ValueError(f"q_start: without it every sequence has one token (got {tokens} tokens, {B} sequences)")
-    return (_lib.PagedCache(k_cache.data_ptr(), v_cache.data_ptr(), k0, k1, k2, v0, v1, v2, pages, rows, heads, dim), heads,
-            dim, _lib.PagedBatch(page_table.data_ptr(), t0, width, q_start, kv_len.data_ptr(), B, tokens, max_q, max_kv))
+    return (_lib.PagedCache.pack(k_cache.data_ptr(), v_cache.data_ptr(), k0, k1, k2, v0, v1, v2, pages, rows, heads, dim), heads,
+            dim, _lib.PagedBatch.pack(page_table.data_ptr(), t0, width, q_start or 0, kv_len.data_ptr(), B, tokens, max_q, max_kv))
 
 
 def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -436,7 +442,7 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
         Hq = q.shape[1]
         if q_out is None:
             q_out = _result(q)
-            ot = _lib.Tokens(q_out.data_ptr(), Hq * D, D)
+            ot = _lib.Tokens.pack(q_out.data_ptr(), Hq * D, D)
         else:
             ot = _tokens(q_out, "q_out", Hq, D, T, dev)
     elif q_out is not None:
@@ -468,7 +474,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     Hq = q.shape[1]
     if out is None:
         out = _result(q)
-        ot = _lib.Tokens(out.data_ptr(), Hq * D, D)
+        ot = _lib.Tokens.pack(out.data_ptr(), Hq * D, D)
     else:
         ot = _tokens(out, "out", Hq, D, T, dev)
     if scale is None:

@@ -265,3 +265,10 @@ def test_workspace_refused():
 def test_plan_refused(kw):
     with pytest.raises(_lib.PolyKernelError, match="pk_paged_attention_plan"):
         attention_plan(**kw)
+
+
+def test_packed_structures_are_the_structures():
+    """The bytes that the front end passes are those of the ctypes structures, whose fields are the header's."""
+    for cls in (_lib.Rotary, _lib.Tokens, _lib.PagedCache, _lib.PagedBatch):
+        values = [0.5 if t is C.c_float else 3 * i + 1 for i, (_, t) in enumerate(cls._fields_)]
+        assert cls.pack(*values) == bytes(cls(*values)) and len(cls.pack(*values)) == C.sizeof(cls)
